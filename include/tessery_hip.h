@@ -50,7 +50,25 @@ int mi_begin(void *runtime);
  * linear4_32x32_k64, linear4_small3, gated4_16x32_k64, gated4_8x32, silu_gate, matmul_f32,
  * matmul_f32_tiled, matmul_f32_chunk32, matmul_bias_f32, matmul_bias_f32_chunk32, add_bias,
  * gelu_f32, layer_norm, add, embedding4, embedding_position, pool_project; additions:
- * attention_f16, attention_f16_scalar, attention_f16_norm_rope, norm_rope_f16, qkv4_f16, copy. */
+ * attention_f16, attention_f16_scalar, attention_f16_norm_rope, norm_rope_f16, qkv4_f16, copy, and, for
+ * packed batches and other encoders (an output that is one of the op's inputs is refused, but where
+ * stated; a buffer that no flag asks for is not read and may be any):
+ *   attention_masked  buffers q, k, v, lengths u32 [B], out, spans u32 [B,S,2], bias f32, prefix u32 [B];
+ *       threads = tokens, group 256; heads, kv_heads, seq, dim (a multiple of 8 to 256), scale;
+ *       u0 0 causal, 1 bidirectional, 2 prefix; u1 bits: 1 fp16 operands and output (else fp32),
+ *       2 spans, 4 bias is slopes [H], 8 bias is tables [H, 2 rows + 1], 16 q and k lie in one buffer
+ *       of rows (H + 2 KV) dim, 32 v lies in such a buffer; n the window (0: none), rows the tables'
+ *       radius, theta the cap (0: none).
+ *   rotary  buffers q, k, positions u32 [tokens], table f32 [positions][k], q_norm and k_norm bf16 [dim],
+ *       q_out, k_out; threads = tokens, group 256; heads, kv_heads (0: q alone), seq, dim, k the rotated
+ *       channels, eps; u0 0 half, 1 interleaved; u1 bits: 1 fp16 (else fp32), 2 positions, 4 norms, 8 q
+ *       and k lie in one buffer of rows (heads + 2 kv_heads) dim, 16 so do q_out and k_out. An output
+ *       may be its own input, in the same layout.
+ *   rotary_table  buffers frequencies f64 [dim / 2], table f32 [n][dim]; threads = n * dim / 2, group 256;
+ *       scale a factor on the entries: dim / 2 cosines of position * frequency, then the sines.
+ *   linear_f16  buffers x f16 [rows, k], w f16 [cols, k], bias f32 [cols], residual f16 [rows, cols], out;
+ *       threads = rows, group 256; u0 the activation (0 none, 1 relu, 2 gelu, 3 gelu by tanh, 4 silu); u1
+ *       bits: 1 bias, 2 residual, 4 out is fp32 (else fp16). A fp16 out may be the residual. */
 int mi_dispatch(void *runtime, const char *name, void **buffers, uint32_t count,
                 const void *parameters, uint32_t size, uint64_t threads, uint32_t group);
 /* runtime.mm:217-253 */

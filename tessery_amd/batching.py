@@ -7,10 +7,12 @@ the reference's for every input, so the policy itself is unchanged; the code is 
 
 from __future__ import annotations
 
-from collections.abc import Iterator
+from collections.abc import Iterator, Sequence
 
 import numpy as np
 from numpy.typing import NDArray
+
+from .errors import InferenceError
 
 PADDED_ARCHITECTURES = ("qwen3_uint4", "bert_f32")
 
@@ -82,3 +84,37 @@ def execution_batches(
         ):
             width = _round_up(width, 4)
         yield rows, width
+
+
+# ---- packed rows: several documents in one batch row -------------------------------------------
+
+
+def _document_bounds(
+    documents: Sequence[Sequence[int]], seq: int
+) -> Iterator[tuple[int, int, int]]:
+    for row, lengths in enumerate(documents):
+        at = 0
+        for length in lengths:
+            if length < 0 or at + length > seq:
+                raise InferenceError()
+            yield row, at, at + length
+            at += length
+
+
+def document_spans(documents: Sequence[Sequence[int]], seq: int) -> NDArray[np.uint32]:
+    """[rows, seq, 2]: for each token the first token of its document and the one behind its last
+    (HipRuntime._attention_masked's spans). documents holds, for each batch row, the lengths of the
+    documents that lie in it one after the other; tokens behind them get empty spans."""
+    spans = np.zeros((len(documents), seq, 2), np.uint32)
+    for row, start, end in _document_bounds(documents, seq):
+        spans[row, start:end] = (start, end)
+    return spans
+
+
+def document_positions(documents: Sequence[Sequence[int]], seq: int) -> NDArray[np.uint32]:
+    """[rows, seq]: each token's index in its document (HipRuntime._rotary's positions), 0 behind
+    the documents."""
+    positions = np.zeros((len(documents), seq), np.uint32)
+    for row, start, end in _document_bounds(documents, seq):
+        positions[row, start:end] = np.arange(end - start)
+    return positions

@@ -243,4 +243,62 @@ hipError_t launch_pool_project_f32(const float* x, const uint32_t* lengths, floa
 // Plain device copy (bytes % 16 == 0), used to calibrate HBM traffic counters.
 hipError_t launch_copy(const void* src, void* dst, uint64_t bytes, hipStream_t st);
 
+// Attention whose scores and keys depend on more than the two operands (route attention_masked). q, k
+// and v point at their first head's first channel, `*_row` elements from token to token (the rows of a
+// q, k and v projection, or tensors of their own); out is [B,S,H,D] of the operands' type.
+enum MaskKind : int { kMaskCausal = 0, kMaskBidirectional = 1, kMaskPrefix = 2 };
+enum ScoreBias : int { kBiasNone = 0, kBiasSlopes = 1, kBiasTable = 2 };
+struct MaskedArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const uint32_t* lengths;  // [B]
+  void* out;
+  const uint32_t* spans;   // [B,S,2] first key and the one behind the last of a token, or null
+  const uint32_t* prefix;  // [B], kMaskPrefix
+  const float* bias;       // slopes [H] or tables [H, 2 radius + 1]
+  int B, S, H, KV, D;
+  int q_row, k_row, v_row;
+  float scale, cap;  // cap 0: none
+  int mask, window, radius, bias_kind;  // window 0: none
+  int f16;
+};
+bool attention_masked_fits(uint64_t B, uint64_t S, uint64_t H, uint64_t D);
+hipError_t launch_attention_masked(const MaskedArgs& a, hipStream_t st);
+
+// Rotation by position of the first `rot` channels of q and k heads, after their RMSNorm when the
+// weights are given (route rotary). Rows of `*_row` elements from token to token; y may be x.
+struct RotaryArgs {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const uint32_t* positions;  // [tokens]; null: token % S
+  const float* table;         // [table_rows][rot]: rot / 2 cosines, then rot / 2 sines
+  const uint16_t *q_norm, *k_norm;  // bf16 [D]; both null: no norm
+  uint32_t tokens, S, table_rows;
+  int H, KV, D, rot, interleaved, f16;
+  int in_q_row, in_k_row, out_q_row, out_k_row;
+  float eps;
+};
+bool rotary_fits(uint64_t tokens, uint64_t heads, uint64_t dim);
+hipError_t launch_rotary(const RotaryArgs& a, hipStream_t st);
+// table[p][c] = factor * cos(p * frequencies[c]), table[p][rot / 2 + c] the sine, in float64 and
+// rounded once.
+hipError_t launch_rotary_table(const double* frequencies, float* table, uint32_t positions, int rot,
+                               float factor, hipStream_t st);
+
+// out = act(x W^T + bias) + residual over fp16 x [M,K] and W [N,K] with fp32 sums (route linear_f16);
+// out fp16 or fp32 [M,N], bias fp32 [N] and residual fp16 [M,N] where not null. out may be residual.
+enum Activation : int { kActNone, kActRelu, kActGelu, kActGeluTanh, kActSilu, kActCount };
+struct LinearF16Args {
+  const _Float16* x;
+  const _Float16* w;
+  const float* bias;
+  const _Float16* residual;
+  void* out;
+  int M, N, K, act, out_f32;
+  float* scratch;  // partial sums
+  size_t scratch_floats;
+};
+hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st);
+
 }  // namespace tessery

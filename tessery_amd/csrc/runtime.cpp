@@ -66,6 +66,10 @@ enum Route : int {
   R_EMBEDDING_POSITION,
   R_POOL_PROJECT,
   R_COPY,
+  R_ATTENTION_MASKED,
+  R_ROTARY,
+  R_ROTARY_TABLE,
+  R_LINEAR_F16,
   R_NONE
 };
 
@@ -109,6 +113,10 @@ const RouteName kRoutes[] = {
     {"embedding_position", R_EMBEDDING_POSITION, 5},
     {"pool_project", R_POOL_PROJECT, 3},
     {"copy", R_COPY, 2},
+    {"attention_masked", R_ATTENTION_MASKED, 8},
+    {"rotary", R_ROTARY, 8},
+    {"rotary_table", R_ROTARY_TABLE, 2},
+    {"linear_f16", R_LINEAR_F16, 5},
 };
 
 Route find_route(const char* name, uint32_t* nbuf) {
@@ -381,6 +389,190 @@ bool matmul_range(Route r, const Params& p, uint64_t threads, uint32_t group, Ro
   return out->r0 < out->r1;
 }
 
+// u1 flags of the routes on packed batches (tessery_hip.h)
+enum MaskedFlag : uint32_t { kMaskedF16 = 1, kMaskedSpans = 2, kMaskedSlopes = 4, kMaskedTable = 8,
+                             kMaskedPackedQk = 16, kMaskedPackedV = 32, kMaskedFlags = 63 };
+enum RotaryFlag : uint32_t { kRotaryF16 = 1, kRotaryPositions = 2, kRotaryNorm = 4,
+                             kRotaryPackedIn = 8, kRotaryPackedOut = 16, kRotaryFlags = 31 };
+enum LinearFlag : uint32_t { kLinearBias = 1, kLinearResidual = 2, kLinearF32 = 4,
+                             kLinearFlags = 7 };
+constexpr uint64_t kMaxSeq = 1u << 20;
+
+// Kernel arguments of an attention_masked op: buffers q, k, v, lengths, out, spans, bias, prefix (those
+// a flag or the mask leaves out are not read). False: not a shape that runs.
+bool masked_args(const Params& p, uint64_t threads, uint32_t group, void* const* ptr,
+                 tessery::MaskedArgs* out) {
+  const uint64_t H = p.heads, KV = p.kv_heads, S = p.seq, D = p.dim, tokens = threads;
+  const uint32_t f = p.u1;
+  if (group != 256 || !H || !KV || H % KV || H > 1024 || !S || S > kMaxSeq || !D || tokens % S ||
+      tokens > kMaxTokens || !tessery::attention_masked_fits(tokens / S, S, H, D))
+    return false;
+  if (p.u0 > tessery::kMaskPrefix || (f & ~kMaskedFlags) ||
+      ((f & kMaskedSlopes) && (f & kMaskedTable)) || p.rows > kMaxSeq ||
+      !std::isfinite(p.scale) || !std::isfinite(p.theta) || p.theta < 0.0f)
+    return false;
+  tessery::MaskedArgs a{};
+  const int e = f & kMaskedF16 ? 2 : 4, wide = static_cast<int>((H + 2 * KV) * D);
+  const bool qk = f & kMaskedPackedQk, v = f & kMaskedPackedV;
+  auto at = [&](int i, uint64_t skip) {
+    return static_cast<const char*>(ptr[i]) + skip * D * static_cast<uint64_t>(e);
+  };
+  a.q = ptr[0];
+  a.k = at(1, qk ? H : 0);
+  a.v = at(2, v ? H + KV : 0);
+  a.q_row = qk ? wide : static_cast<int>(H * D);
+  a.k_row = qk ? wide : static_cast<int>(KV * D);
+  a.v_row = v ? wide : static_cast<int>(KV * D);
+  a.lengths = static_cast<const uint32_t*>(ptr[3]);
+  a.out = ptr[4];
+  a.spans = f & kMaskedSpans ? static_cast<const uint32_t*>(ptr[5]) : nullptr;
+  a.bias = f & (kMaskedSlopes | kMaskedTable) ? static_cast<const float*>(ptr[6]) : nullptr;
+  a.prefix = p.u0 == tessery::kMaskPrefix ? static_cast<const uint32_t*>(ptr[7]) : nullptr;
+  a.B = static_cast<int>(tokens / S);
+  a.S = static_cast<int>(S);
+  a.H = static_cast<int>(H);
+  a.KV = static_cast<int>(KV);
+  a.D = static_cast<int>(D);
+  a.scale = p.scale;
+  a.cap = p.theta;
+  a.mask = static_cast<int>(p.u0);
+  a.window = static_cast<int>(std::min<uint64_t>(p.n, S));
+  a.radius = static_cast<int>(p.rows);
+  a.bias_kind = f & kMaskedSlopes  ? tessery::kBiasSlopes
+                : f & kMaskedTable ? tessery::kBiasTable
+                                   : tessery::kBiasNone;
+  a.f16 = e == 2;
+  *out = a;
+  return true;
+}
+
+bool masked_sizes(const tessery::MaskedArgs& a, uint32_t flags, const uint64_t* sz) {
+  const uint64_t e = a.f16 ? 2 : 4, tokens = static_cast<uint64_t>(a.B) * a.S;
+  const uint64_t H = a.H, KV = a.KV, D = a.D, wide = (H + 2 * KV) * D;
+  const uint64_t n[3] = {flags & kMaskedPackedQk ? wide : H * D,
+                         flags & kMaskedPackedQk ? wide : KV * D,
+                         flags & kMaskedPackedV ? wide : KV * D};
+  for (int i = 0; i < 3; ++i)
+    if (sz[i] < tokens * n[i] * e) return false;
+  const uint64_t bias = a.bias_kind == tessery::kBiasSlopes  ? H
+                        : a.bias_kind == tessery::kBiasTable ? H * (2 * uint64_t(a.radius) + 1)
+                                                             : 0;
+  return sz[3] >= a.B * uint64_t{4} && sz[4] >= tokens * H * D * e &&
+         (!(flags & kMaskedSpans) || sz[5] >= tokens * 8) && sz[6] >= bias * 4 &&
+         (a.mask != tessery::kMaskPrefix || sz[7] >= a.B * uint64_t{4});
+}
+
+// Kernel arguments of a rotary op: buffers q, k, positions, table, q_norm, k_norm, q_out, k_out
+// (positions and norms only with their flags, k and k_out only with key heads).
+bool rotary_args(const Params& p, uint64_t threads, uint32_t group, void* const* ptr,
+                 const uint64_t* sz, tessery::RotaryArgs* out) {
+  const uint64_t H = p.heads, KV = p.kv_heads, S = p.seq, D = p.dim, r = p.k, tokens = threads;
+  const uint32_t f = p.u1;
+  if (group != 256 || !H || H > 1024 || KV > 1024 || !S || tokens % S || tokens > kMaxTokens ||
+      !D || !r || r % 2 || r > D || p.u0 > 1 || (f & ~kRotaryFlags) || !(p.eps >= 0.0f) ||
+      !std::isfinite(p.eps) || !tessery::rotary_fits(tokens, H + KV, D) ||
+      ((f & (kRotaryPackedIn | kRotaryPackedOut)) && !KV))
+    return false;
+  const uint64_t e = f & kRotaryF16 ? 2 : 4, wide = (H + 2 * KV) * D;
+  const bool in = f & kRotaryPackedIn, to = f & kRotaryPackedOut, norm = f & kRotaryNorm;
+  const uint64_t n[4] = {in ? wide : H * D, in ? wide : KV * D, to ? wide : H * D,
+                         to ? wide : KV * D};
+  if (sz[0] < tokens * n[0] * e || sz[1] < tokens * n[1] * e || sz[6] < tokens * n[2] * e ||
+      sz[7] < tokens * n[3] * e || ((f & kRotaryPositions) && sz[2] < tokens * 4) ||
+      (norm && (sz[4] < D * 2 || (KV && sz[5] < D * 2))) || sz[3] < r * 4)
+    return false;
+  const uint64_t rows = sz[3] / (r * 4);
+  // without positions the rows of the table that a call reads are known here
+  if (!(f & kRotaryPositions) && rows < S) return false;
+  tessery::RotaryArgs a{};
+  a.q = ptr[0];
+  a.k = static_cast<const char*>(ptr[1]) + (in ? H * D * e : 0);
+  a.q_out = ptr[6];
+  a.k_out = static_cast<char*>(ptr[7]) + (to ? H * D * e : 0);
+  a.positions = f & kRotaryPositions ? static_cast<const uint32_t*>(ptr[2]) : nullptr;
+  a.table = static_cast<const float*>(ptr[3]);
+  a.q_norm = norm ? static_cast<const uint16_t*>(ptr[4]) : nullptr;
+  a.k_norm = norm ? static_cast<const uint16_t*>(ptr[5]) : nullptr;
+  a.tokens = static_cast<uint32_t>(tokens);
+  a.S = static_cast<uint32_t>(S);
+  a.table_rows = static_cast<uint32_t>(std::min<uint64_t>(rows, 0xffffffffull));
+  a.H = static_cast<int>(H);
+  a.KV = static_cast<int>(KV);
+  a.D = static_cast<int>(D);
+  a.rot = static_cast<int>(r);
+  a.interleaved = static_cast<int>(p.u0);
+  a.f16 = e == 2;
+  a.in_q_row = static_cast<int>(n[0]);
+  a.in_k_row = static_cast<int>(n[1]);
+  a.out_q_row = static_cast<int>(n[2]);
+  a.out_k_row = static_cast<int>(n[3]);
+  a.eps = p.eps;
+  *out = a;
+  return true;
+}
+
+// Kernel arguments of a linear_f16 op: buffers x, w, bias, residual, out (bias and residual only with
+// their flags).
+bool linear_f16_args(const Params& p, uint64_t threads, uint32_t group, void* const* ptr,
+                     const uint64_t* sz, tessery::LinearF16Args* out) {
+  const uint64_t M = p.rows, N = p.cols, K = p.k;
+  const uint32_t f = p.u1;
+  if (group != 256 || threads != M || !M || M > (1u << 22) || !N || N > 65536 || !K ||
+      K > 65536 || p.u0 >= tessery::kActCount || (f & ~kLinearFlags))
+    return false;
+  if (sz[0] < M * K * 2 || sz[1] < N * K * 2 || ((f & kLinearBias) && sz[2] < N * 4) ||
+      ((f & kLinearResidual) && sz[3] < M * N * 2) || sz[4] < M * N * (f & kLinearF32 ? 4 : 2))
+    return false;
+  tessery::LinearF16Args a{};
+  a.x = static_cast<const _Float16*>(ptr[0]);
+  a.w = static_cast<const _Float16*>(ptr[1]);
+  a.bias = f & kLinearBias ? static_cast<const float*>(ptr[2]) : nullptr;
+  a.residual = f & kLinearResidual ? static_cast<const _Float16*>(ptr[3]) : nullptr;
+  a.out = ptr[4];
+  a.M = static_cast<int>(M);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.act = static_cast<int>(p.u0);
+  a.out_f32 = f & kLinearF32 ? 1 : 0;
+  *out = a;
+  return true;
+}
+
+// Whether no output of an op of these routes is a buffer that it still reads when the output is
+// written. Other routes take their buffers as they come.
+bool outputs_apart(Route r, const Params& p, void* const* ptr) {
+  switch (r) {
+    case R_ATTENTION_MASKED:
+      for (int i = 0; i < 8; ++i)
+        if (i != 4 && ptr[i] == ptr[4]) return false;
+      return !(p.u1 & kMaskedPackedQk) || ptr[0] == ptr[1];
+    case R_ROTARY: {
+      const bool in = p.u1 & kRotaryPackedIn, to = p.u1 & kRotaryPackedOut;
+      // packed rows hold q and k; a row may only be rotated where it lies
+      if ((in && ptr[0] != ptr[1]) || (to && ptr[6] != ptr[7])) return false;
+      if (!to && p.kv_heads && ptr[6] == ptr[7]) return false;
+      for (int o = 6; o < 8; ++o) {
+        if (o == 7 && !p.kv_heads) break;
+        for (int i = 0; i < 6; ++i) {
+          if (ptr[i] != ptr[o]) continue;
+          const bool own = in && to ? i < 2 : !in && !to && i == o - 6;
+          if (!own && !(i == 1 && !p.kv_heads)) return false;
+        }
+      }
+      return true;
+    }
+    case R_ROTARY_TABLE:
+      return ptr[0] != ptr[1];
+    case R_LINEAR_F16:
+      // out may be the residual (each element is read, then written, by one thread) of its type
+      for (int i = 0; i < 3; ++i)
+        if (ptr[i] == ptr[4]) return false;
+      return ptr[3] != ptr[4] || ((p.u1 & kLinearResidual) && !(p.u1 & kLinearF32));
+    default:
+      return true;
+  }
+}
+
 // Validates one launch against the buffer sizes it would touch. Pure: no allocation.
 bool validate(Route r, const Params& p, uint64_t threads, uint32_t group, const uint64_t* sz,
               uint32_t count, uint32_t nbuf) {
@@ -536,6 +728,27 @@ bool validate(Route r, const Params& p, uint64_t threads, uint32_t group, const 
     }
     case R_COPY:
       return threads % 16 == 0 && sz[0] >= threads && sz[1] >= threads;
+    case R_ATTENTION_MASKED: {
+      void* const none[kMaxBuffers] = {};
+      tessery::MaskedArgs a;
+      return masked_args(p, threads, group, none, &a) && masked_sizes(a, p.u1, sz);
+    }
+    case R_ROTARY: {
+      void* const none[kMaxBuffers] = {};
+      tessery::RotaryArgs a;
+      return rotary_args(p, threads, group, none, sz, &a);
+    }
+    case R_ROTARY_TABLE: {  // buffers: frequencies f64 [dim / 2], table f32 [n, dim]
+      const uint64_t n = p.n, r = p.dim;
+      return group == 256 && n && r && r % 2 == 0 && r <= 1024 && threads == n * (r / 2) &&
+             threads <= kMaxElements && std::isfinite(p.scale) && sz[0] >= r / 2 * 8 &&
+             sz[1] >= n * r * 4;
+    }
+    case R_LINEAR_F16: {
+      void* const none[kMaxBuffers] = {};
+      tessery::LinearF16Args a;
+      return linear_f16_args(p, threads, group, none, sz, &a);
+    }
     default:
       return false;
   }
@@ -871,6 +1084,29 @@ hipError_t launch(Runtime* rt, const Op& op, const Beside& beside) {
           p.dim, p.u1 != 0, st);
     case R_COPY:
       return tessery::launch_copy(op.ptr[0], op.ptr[1], op.threads, st);
+    case R_ATTENTION_MASKED: {
+      tessery::MaskedArgs a;
+      if (!masked_args(p, op.threads, op.group, op.ptr.data(), &a)) return hipErrorInvalidValue;
+      return tessery::launch_attention_masked(a, st);
+    }
+    case R_ROTARY: {
+      tessery::RotaryArgs a;
+      if (!rotary_args(p, op.threads, op.group, op.ptr.data(), op.size.data(), &a))
+        return hipErrorInvalidValue;
+      return tessery::launch_rotary(a, st);
+    }
+    case R_ROTARY_TABLE:
+      return tessery::launch_rotary_table(static_cast<const double*>(op.ptr[0]),
+                                          static_cast<float*>(op.ptr[1]), p.n,
+                                          static_cast<int>(p.dim), p.scale, st);
+    case R_LINEAR_F16: {
+      tessery::LinearF16Args a;
+      if (!linear_f16_args(p, op.threads, op.group, op.ptr.data(), op.size.data(), &a))
+        return hipErrorInvalidValue;
+      a.scratch = rt->dense_scratch;
+      a.scratch_floats = kDenseScratchFloats;
+      return tessery::launch_linear_f16(a, st);
+    }
     default:
       return hipErrorInvalidValue;
   }
@@ -1033,7 +1269,7 @@ int mi_dispatch(void* runtime, const char* name, void** buffers, uint32_t count,
     ptrs[i] = b->ptr;
     sizes[i] = b->size;
   }
-  if (!validate(r, p, threads, group, sizes, count, nbuf)) return 1;
+  if (!validate(r, p, threads, group, sizes, count, nbuf) || !outputs_apart(r, p, ptrs)) return 1;
   Op op;
   make_op(r, p, threads, group, ptrs, sizes, count, &op);
   if (hipSetDevice(rt->device) != hipSuccess || !prepare(rt, op)) return 1;
@@ -1839,6 +2075,7 @@ int mi_plan_run(void* runtime, void* plan, void** buffers, uint32_t count) {
       ptrs[i] = b->ptr;
       sizes[i] = b->size;
     }
+    if (!outputs_apart(po.route, po.p, ptrs)) return 1;
     Op op;
     make_op(po.route, po.p, po.threads, po.group, ptrs, sizes, po.count, &op);
     if (!prepare(rt, op)) return 1;

@@ -14,6 +14,9 @@ Additions, all keyword-only with defaults that keep the reference behaviour:
   * `_attention(..., precision="f16", out_dtype=...)`: fp16 operands, fp32 accumulation on MFMA;
   * `_attention_norm_rope(...)`: the Qwen3 q/k RMSNorm + RoPE fused into the fp16 attention;
   * `_qkv4(...)`: the three uint4 QKV projections of fp16 activations in one launch;
+  * `_attention_masked(...)`, `_rotary(...)`, `_rotary_table(...)`, `_linear_f16(...)`: attention with
+    capped or biased scores and prefix, window and document masks, rotary positions of other layouts
+    and lengths, and fp16 projections with their epilogue, for encoders other than the two here;
   * `read(..., dtype=...)` for fp16 buffers, `write` and `upload`.
 
 Structure of the host side:
@@ -35,6 +38,7 @@ from __future__ import annotations
 
 import ctypes as ct
 import hashlib
+import math
 import struct
 import threading
 import time
@@ -238,6 +242,87 @@ def attention_norm_rope_plan(*, tokens: int, seq: int, heads: int, kv_heads: int
                     theta=theta, bidirectional=bidirectional, out_f16=out_f16),
                slots=(0, 7, 2, 3, 4, 5)),
     ]
+
+
+# Head dimensions of attention_masked: multiples of 8 up to this.
+MASKED_MAX_DIM = 256
+MASKS = {"causal": 0, "bidirectional": 1, "prefix": 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+_F16_FLAG = {"f32": 0, "f16": 1}
+
+
+def _sized(*values: Any) -> bool:
+    """Whether every value is a positive int."""
+    return all(type(v) is int and v > 0 for v in values)
+
+
+def attention_masked_plan(*, tokens: int, seq: int, heads: int, kv_heads: int, dim: int,
+                          mask: str = "causal", window: int = 0, cap: float = 0.0,
+                          radius: int = 0, scale: float | None = None, precision: str = "f16",
+                          packed: bool | str = False, spans: bool = False, slopes: bool = False,
+                          table: bool = False, prefix: bool = False) -> list[Launch]:
+    """The one launch of _attention_masked over buffers [q, k, v, lengths, out, spans, bias,
+    prefix]; spans, slopes, table and prefix say which of the last three are there, and lengths
+    stands in for the others. Params: u0 the mask, u1 the flags, n the window, rows the table's
+    radius, theta the cap."""
+    if not _sized(tokens, seq, heads, kv_heads, dim) or tokens % seq or heads % kv_heads or \
+            dim % 8 or dim > MASKED_MAX_DIM:
+        raise InferenceError()
+    if mask not in MASKS or precision not in _F16_FLAG or packed not in (False, True, "v") or \
+            (mask == "prefix") != prefix or (slopes and table):
+        raise InferenceError()
+    if type(window) is not int or not 0 <= window < 2**32 or type(radius) is not int or \
+            not 0 <= radius <= 2**20 or (radius and not table):
+        raise InferenceError()
+    scale = dim**-0.5 if scale is None else float(scale)
+    cap = float(cap)
+    if not math.isfinite(scale) or not 0.0 <= cap < 3.4e38:
+        raise InferenceError()
+    flags = (_F16_FLAG[precision] | 2 * spans | 4 * slopes | 8 * table | 16 * (packed is True)
+             | 32 * (packed is not False))
+    here = [spans, slopes or table, prefix]
+    slots = (0, 1, 2, 3, 4) + tuple(5 + i if there else 3 for i, there in enumerate(here))
+    return [Launch("attention_masked", tokens, 256,
+                   dict(seq=seq, heads=heads, kv_heads=kv_heads, dim=dim, scale=scale, theta=cap,
+                        n=window, rows=radius, bidirectional=MASKS[mask], flags=flags), slots)]
+
+
+def rotary_plan(*, tokens: int, seq: int, heads: int, kv_heads: int, dim: int, rotary_dim: int,
+                layout: str = "half", precision: str = "f16", eps: float = 1e-6,
+                packed: bool = False, packed_out: bool = False, positions: bool = False,
+                norm: bool = False) -> list[Launch]:
+    """The one launch of _rotary over buffers [q, k, table, q_out, k_out, positions, q_norm,
+    k_norm]; positions and norm say which of the last three are there, and the table stands in for
+    the others (and for k and k_out where there are no key heads)."""
+    if not _sized(tokens, seq, heads, dim, rotary_dim) or tokens % seq or \
+            type(kv_heads) is not int or kv_heads < 0 or rotary_dim % 2 or rotary_dim > dim or \
+            dim > 1024:
+        raise InferenceError()
+    if layout not in ROTARY_LAYOUTS or precision not in _F16_FLAG or not 0.0 <= eps < 3.4e38 or \
+            ((packed or packed_out) and not kv_heads):
+        raise InferenceError()
+    flags = (_F16_FLAG[precision] | 2 * positions | 4 * norm | 8 * bool(packed)
+             | 16 * bool(packed_out))
+    k, k_out = (1, 4) if kv_heads else (2, 2)
+    slots = (0, k, 5 if positions else 2, 2, 6 if norm else 2, 7 if norm and kv_heads else 2, 3,
+             k_out)
+    return [Launch("rotary", tokens, 256,
+                   dict(seq=seq, heads=heads, kv_heads=kv_heads, dim=dim, k=rotary_dim, eps=eps,
+                        bidirectional=ROTARY_LAYOUTS[layout], flags=flags), slots)]
+
+
+def linear_f16_plan(*, rows: int, cols: int, k: int, activation: str = "none",
+                    out_dtype: str = "f16", bias: bool = False,
+                    residual: bool = False) -> list[Launch]:
+    """The one launch of _linear_f16 over buffers [x, w, out, bias, residual]; bias and residual
+    say which of the last two are there, and x stands in for the others."""
+    if not _sized(rows, cols, k) or activation not in ACTIVATIONS or out_dtype not in _F16_FLAG:
+        raise InferenceError()
+    flags = bias | 2 * residual | 4 * (out_dtype == "f32")
+    return [Launch("linear_f16", rows, 256,
+                   dict(rows=rows, cols=cols, k=k, bidirectional=ACTIVATIONS[activation],
+                        flags=flags), (0, 1, 3 if bias else 0, 4 if residual else 0, 2))]
 
 
 def linear4_plan(*, rows: int, cols: int, k: int) -> list[Launch]:
@@ -891,6 +976,90 @@ class HipRuntime:
             raise InferenceError()
         self._dispatch("qkv4_f16", buffers, threads=rows, group_size=256, rows=rows, k=k,
                        cols=q_cols, n=kv_cols, flags=flag)
+
+    def _attention_masked(self, buffers: Sequence[Buffer], *, tokens: int, seq: int, heads: int,
+                          kv_heads: int, dim: int, mask: str = "causal", window: int = 0,
+                          cap: float = 0.0, scale: float | None = None, precision: str = "f16",
+                          packed: bool | str = False, prefix: Buffer | None = None,
+                          spans: Buffer | None = None, slopes: Buffer | None = None,
+                          table: Buffer | None = None, radius: int = 0) -> None:
+        """Attention whose scores and keys depend on more than q and k; buffers = [q, k, v, lengths
+        (u32 [batch]), out], fp16 or fp32 (`precision`) as _attention lays them out, out of the same
+        type. dim is a multiple of 8 up to 256.
+
+        Scores are scale * q.k (scale: dim^-0.5 unless given), then cap * tanh(score / cap) with a
+        cap > 0, then less slopes[head] * |i - j| (fp32 [heads]) or plus
+        table[head, clamp(j - i, -radius, radius) + radius] (fp32 [heads, 2 * radius + 1]).
+
+        Token i of a batch row attends the keys j below the row's length that `mask` leaves -
+        "causal" j <= i, "bidirectional" all, "prefix" j <= i or j < prefix[row] (u32 [batch]) -
+        and that satisfy |i - j| < window (0: no window) and
+        spans[row, i, 0] <= j < spans[row, i, 1] (u32 [batch, seq, 2], the documents of packed rows:
+        batching.document_spans). A token that attends no key gets zeros. Rows at or past the length
+        are outputs like any other. Infinities and NaN of keys and values reach only the tokens
+        that attend them.
+
+        packed: q, k and v are one buffer (given three times) whose rows hold the heads of q, k and
+        v; "v": only v lies in such rows."""
+        if len(buffers) != 5:
+            raise InferenceError()
+        plan = attention_masked_plan(
+            tokens=tokens, seq=seq, heads=heads, kv_heads=kv_heads, dim=dim, mask=mask,
+            window=window, cap=cap, radius=radius, scale=scale, precision=precision,
+            packed=packed, spans=spans is not None, slopes=slopes is not None,
+            table=table is not None, prefix=prefix is not None)
+        _run_plan(self, [*buffers, spans, slopes if slopes is not None else table, prefix], plan)
+
+    def _rotary(self, buffers: Sequence[Buffer | None], *, tokens: int, seq: int, heads: int,
+                kv_heads: int, dim: int, rotary_dim: int, layout: str = "half",
+                precision: str = "f16", packed: bool = False, positions: Buffer | None = None,
+                q_norm: Buffer | None = None, k_norm: Buffer | None = None,
+                eps: float = 1e-6) -> None:
+        """Rotation of q and k by position, after their per-head RMSNorm where q_norm and k_norm
+        (bf16 [dim]) are given; buffers = [q [tokens, heads, dim], k [tokens, kv_heads, dim], table,
+        q_out, k_out], fp16 or fp32 (`precision`), table as rotary.table makes it (fp32 [positions,
+        rotary_dim]). The first rotary_dim channels of a head turn, in pairs (c, c + rotary_dim / 2)
+        ("half") or (2c, 2c + 1) ("interleaved"); the others keep their normed values. q_out and
+        k_out may be q and k. kv_heads = 0: only q (k and k_out None).
+
+        positions: u32 [tokens] (documents of packed rows: batching.document_positions); without
+        them a token's index in its row of seq tokens. A position behind the table gives zeros.
+
+        packed: q and k are one buffer whose rows hold the heads of q, k and v (kv_heads of v); so
+        are q_out and k_out when they are that buffer, else they hold q and k alone."""
+        if len(buffers) != 5 or (q_norm is None) != (k_norm is None) and (kv_heads or k_norm):
+            raise InferenceError()
+        q, k, table, q_out, k_out = buffers
+        same = packed and q_out is q and k_out is k
+        plan = rotary_plan(tokens=tokens, seq=seq, heads=heads, kv_heads=kv_heads, dim=dim,
+                           rotary_dim=rotary_dim, layout=layout, precision=precision, eps=eps,
+                           packed=packed, packed_out=same, positions=positions is not None,
+                           norm=q_norm is not None)
+        _run_plan(self, [q, k, table, q_out, k_out, positions, q_norm, k_norm], plan)
+
+    def _rotary_table(self, buffers: Sequence[Buffer], *, positions: int, rotary_dim: int,
+                      factor: float = 1.0) -> None:
+        """The table _rotary reads; buffers = [frequencies (float64 [rotary_dim / 2], radians a
+        position), table (fp32 [positions, rotary_dim])]. The cosines and sines of
+        position * frequency are taken in float64 and multiplied by `factor`."""
+        if len(buffers) != 2 or not _sized(positions, rotary_dim) or rotary_dim % 2 or \
+                not math.isfinite(factor):
+            raise InferenceError()
+        self._dispatch("rotary_table", buffers, threads=positions * (rotary_dim // 2),
+                       group_size=256, n=positions, dim=rotary_dim, scale=factor)
+
+    def _linear_f16(self, buffers: Sequence[Buffer], *, rows: int, cols: int, k: int,
+                    bias: Buffer | None = None, residual: Buffer | None = None,
+                    activation: str = "none", out_dtype: str = "f16") -> None:
+        """out = act(x w^T + bias) + residual for fp16 activations and weights; buffers = [x [rows,
+        k], w [cols, k], out [rows, cols]], bias fp32 [cols], residual fp16 [rows, cols], out fp16
+        or fp32 (`out_dtype`). activation: "none", "relu", "gelu" (with erf), "gelu_tanh" or
+        "silu". Sums and epilogue are fp32, rounded once. A fp16 out may be the residual."""
+        if len(buffers) != 3:
+            raise InferenceError()
+        _run_plan(self, [*buffers, bias, residual], linear_f16_plan(
+            rows=rows, cols=cols, k=k, activation=activation, out_dtype=out_dtype,
+            bias=bias is not None, residual=residual is not None))
 
     def _linear4(self, buffers: Sequence[Buffer], *, rows: int, cols: int, k: int) -> None:
         """uint4 projection [x, w, scales, biases, out] over the route partition of
