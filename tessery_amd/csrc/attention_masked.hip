@@ -92,6 +92,370 @@ __device__ __forceinline__ void masked_row(const MaskedArgs& a, int b, int i, in
     if (lane + 64 * c < a.D) out[lane + 64 * c] = static_cast<T>(acc[c] * inv);
 }
 
+// 8 bytes of a row-major fp16 V tile a lane, transposed across each group of 16 lanes: lane r of a group
+// names row r / 4, channels 4 (r % 4) .. + 3 and receives channel r of the four rows.
+typedef __fp16 fp16x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ half4 read_transposed(const _Float16* p) {
+  const fp16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+      (__attribute__((address_space(3))) fp16x4_t*)(p));
+  return __builtin_bit_cast(half4, v);
+}
+
+// The hardware does not hold back a VALU read of an MFMA result and the compiler pads such reads only
+// inside a basic block: 20 wait states (a 32x32x16 product needs 19) before a branch may follow.
+__device__ __forceinline__ void product_done(floatx16& acc) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(acc));
+}
+
+__device__ __forceinline__ float other_half(float x, bool take_max) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float a = __uint_as_float(p[0]), b = __uint_as_float(p[1]);
+  return take_max ? fmaxf(a, b) : a + b;
+}
+
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off));
+  return x;
+}
+__device__ __forceinline__ int wave_max_int(int x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x = max(x, __shfl_xor(x, off));
+  return x;
+}
+
+// Keys that some row of a wavefront attends (lo, hi) and keys that all its rows attend (all_lo, all_hi).
+struct WaveKeys {
+  int lo, hi, all_lo, all_hi;
+};
+
+__device__ __forceinline__ WaveKeys wave_keys(KeyRange r, bool row) {
+  const bool some = row && r.lo < r.hi;
+  WaveKeys w;
+  w.lo = wave_min(some ? r.lo : 0x7fffffff);
+  w.hi = wave_max_int(some ? r.hi : 0);
+  w.all_lo = wave_max_int(!row ? 0 : some ? r.lo : 0x7fffffff);
+  w.all_hi = wave_min(!row ? 0x7fffffff : some ? r.hi : 0);
+  return w;
+}
+
+// The running maximum of a row moves when a tile exceeds it by more than kSlack (log2 units), and
+// probabilities carry 2^kLift: at most 2^14 in fp16, and full fp16 precision down to 2^-20 of the
+// largest. The softmax does not depend on either.
+constexpr float kSlack = 8.0f, kLift = 6.0f;
+
+// What the kernels on tiles take beside the arguments: signs and factors of the scores in log2 units.
+struct ScoreArgs {
+  float q_sign;  // -1 for a negative scale, 0 for none
+  float scale2;  // |scale| log2 e; with a cap the factor in front of tanh's exponent, 2 |scale| log2 e / cap
+  float cap2;    // cap log2 e
+};
+
+// Scores of one 32-key block as v (log2 units), still to be masked: element e of lane (query, h) is the
+// key 8 (e / 4) + 4 h + e % 4 of the block. rel: the key of element 0 less the query's position.
+template <bool CAP, int BIAS>
+__device__ __forceinline__ void score_block(floatx16& v, const ScoreArgs& s, float slope2, float rel,
+                                            const float* biases) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int c = 8 * (e >> 2) + (e & 3);
+    float x = v[e];
+    if constexpr (CAP) {
+      // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0
+      const float t = __builtin_amdgcn_exp2f(x * s.scale2);
+      x = fmaf(-2.0f * s.cap2, __builtin_amdgcn_rcpf(t + 1.0f), s.cap2);
+    } else if constexpr (BIAS != kBiasNone) {
+      x *= s.scale2;
+    }
+    if constexpr (BIAS == kBiasSlopes) x = fmaf(-slope2, fabsf(rel + static_cast<float>(c)), x);
+    if constexpr (BIAS == kBiasTable) x += biases[c];
+    v[e] = x;
+  }
+}
+
+// Tiles of fp16 operands on v_mfma_f32_32x32x16_f16: lane (r = l % 32, h = l / 32) supplies A[r][8h ..
+// 8h + 7] and B[8h .. 8h + 7][r] and holds D[8a + 4h + c][r] in element 4a + c.
+//   S^T = K Q^T for blocks of 32 keys x 32 queries: a query's scores lie in the two lanes r and r + 32.
+//   O^T = V^T P^T for 16 keys x 32 channels at a time: a lane's probabilities 8s .. 8s + 7 (keys 16s + 4h
+//   .. + 3 and 16s + 8 + 4h .. + 3) are the B operand as they lie; the A operand takes the same keys of V
+//   by two transposed reads.
+// Four wavefronts: 4 / KS of them take 32 queries each and the KS groups every KS-th block of keys; the
+// groups' sums meet in LDS at the end. K and V tiles of KT keys pass through registers into two LDS
+// buffers, the next tile's loads in flight during the products; keys past the length become zeros.
+// DP: the head size up to a power of two, zeros behind D.
+template <int DP>
+struct F16Tile {
+  static constexpr int KT = DP == 256 ? 32 : 64;
+  static constexpr int KROW = DP + 8;             // halves: 16 rows' chunks fall on 16 bank groups
+  static constexpr int K = KT * KROW, V = KT * DP;
+  static constexpr int CHUNKS = KT * DP / 8 / 256;  // 16-byte pieces a thread stages of K (and of V)
+  static constexpr int BIASES = 192;              // distances of one tile, KT + 128 - 1
+  static constexpr int BYTES = 2 * (K + V) * 2 + 2 * BIASES * 4;
+};
+// 64-byte units of a V row, so that the four rows of a transposed read fall on different banks
+template <int DP>
+__device__ __forceinline__ int v_unit(int row) {
+  return DP >= 128 ? (row & 3) : DP == 64 ? ((row >> 1) & 1) : 0;
+}
+
+template <int DP, int KS, bool CAP, int BIAS>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(MaskedArgs a, ScoreArgs sc) {
+  using T = F16Tile<DP>;
+  constexpr int KT = T::KT, QW = 4 / KS, QB = 32 * QW, NS = DP / 16, NDT = DP / 32;
+  constexpr int NB = KT / 32 / KS;  // key blocks of a tile that one wavefront takes
+  static_assert(NB >= 1, "a block of keys for every group");
+  __shared__ __attribute__((aligned(16))) char lds[T::BYTES];
+  __shared__ int ends[4][2];
+  _Float16* const kt0 = reinterpret_cast<_Float16*>(lds);
+  _Float16* const vt0 = kt0 + 2 * T::K;
+  float* const bt0 = reinterpret_cast<float*>(vt0 + 2 * T::V);
+
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qw = wave % QW, group = wave / QW;
+  const int blocks = (a.S + QB - 1) / QB;
+  // the last (causally longest) blocks of a head first
+  int at = static_cast<int>(blockIdx.x);
+  const int qb = blocks - 1 - at % blocks;
+  at /= blocks;
+  const int head = at % a.H, b = at / a.H;
+  const int kvh = head / (a.H / a.KV);
+  const int i0 = qb * QB, i = i0 + qw * 32 + r;
+  const bool row = i < a.S;
+  const int ic = min(i, a.S - 1);
+  const KeyRange mine = key_range(a, b, ic);
+  const WaveKeys wk = wave_keys(mine, row);
+  if (lane == 0) {
+    ends[wave][0] = wk.lo;
+    ends[wave][1] = wk.hi;
+  }
+  const int L = static_cast<int>(min(a.lengths[b], static_cast<uint32_t>(a.S)));
+  const size_t token = static_cast<size_t>(b) * a.S;
+  const _Float16* const q = static_cast<const _Float16*>(a.q) + (token + ic) * a.q_row + head * a.D;
+  const _Float16* const k = static_cast<const _Float16*>(a.k) + token * a.k_row + kvh * a.D;
+  const _Float16* const v = static_cast<const _Float16*>(a.v) + token * a.v_row + kvh * a.D;
+
+  half8 qf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    qf[s] = half8{};
+    if (16 * s + 8 * h < a.D) {
+      qf[s] = *reinterpret_cast<const half8*>(q + 16 * s + 8 * h);
+      if (sc.q_sign != 1.0f) qf[s] *= static_cast<_Float16>(sc.q_sign);
+    }
+  }
+  const float slope2 = BIAS == kBiasSlopes ? a.bias[head] * kLog2e : 0.0f;
+  const float* const table =
+      BIAS == kBiasTable ? a.bias + head * (2 * static_cast<size_t>(a.radius) + 1) : nullptr;
+  __syncthreads();
+  int lo = ends[0][0], hi = ends[0][1];
+#pragma unroll
+  for (int w = 1; w < QW; ++w) {
+    lo = min(lo, ends[w][0]);
+    hi = max(hi, ends[w][1]);
+  }
+  const int first = lo / KT, last = (hi + KT - 1) / KT;  // hi 0: no tile
+
+  // staging: thread t takes 16-byte pieces t, t + 256, ... of the tile
+  half8 kreg[T::CHUNKS], vreg[T::CHUNKS];
+  float breg = 0.0f;
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int c = 0; c < T::CHUNKS; ++c) {
+      const int piece = tid + 256 * c, key = tile * KT + piece / (DP / 8), ch = piece % (DP / 8) * 8;
+      kreg[c] = vreg[c] = half8{};
+      if (key < L && ch < a.D) {
+        kreg[c] = *reinterpret_cast<const half8*>(k + static_cast<size_t>(key) * a.k_row + ch);
+        vreg[c] = *reinterpret_cast<const half8*>(v + static_cast<size_t>(key) * a.v_row + ch);
+      }
+    }
+    if constexpr (BIAS == kBiasTable) {
+      // entry x: distance key - query of tile * KT - i0 + x - (QB - 1)
+      const int away = tile * KT - i0 + tid - (QB - 1);
+      if (tid < KT + QB - 1) breg = log2_bias(table[min(max(away, -a.radius), a.radius) + a.radius]);
+    }
+  };
+  auto stage = [&](int buffer) {
+    _Float16* const kt = kt0 + buffer * T::K;
+    _Float16* const vt = vt0 + buffer * T::V;
+#pragma unroll
+    for (int c = 0; c < T::CHUNKS; ++c) {
+      const int piece = tid + 256 * c, key = piece / (DP / 8), ch = piece % (DP / 8);
+      *reinterpret_cast<half8*>(kt + key * T::KROW + 8 * ch) = kreg[c];
+      *reinterpret_cast<half8*>(vt + key * DP + 8 * (ch ^ (4 * v_unit<DP>(key)))) = vreg[c];
+    }
+    if constexpr (BIAS == kBiasTable)
+      if (tid < KT + QB - 1) bt0[buffer * T::BIASES + tid] = breg;
+  };
+
+  floatx16 o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+  float top = -INFINITY, base = 0.0f, sum = 0.0f;
+
+  if (first < last) {
+    fetch(first);
+    stage(0);
+  }
+  __syncthreads();
+  for (int tile = first; tile < last; ++tile) {
+    const int buffer = (tile - first) & 1;
+    if (tile + 1 < last) fetch(tile + 1);
+    const _Float16* const kt = kt0 + buffer * T::K;
+    const _Float16* const vt = vt0 + buffer * T::V;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int kb = (KS == 1 ? nb : group) * 32, j0 = tile * KT + kb;
+      if (j0 >= wk.hi || j0 + 32 <= wk.lo) continue;  // wavefront-uniform
+      floatx16 s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        const half8 kf = *reinterpret_cast<const half8*>(kt + (kb + r) * T::KROW + 16 * st + 8 * h);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], s, 0, 0, 0);
+      }
+      product_done(s);
+      score_block<CAP, BIAS>(s, sc, slope2, static_cast<float>(j0 + 4 * h - i),
+                             bt0 + buffer * T::BIASES + kb + 4 * h + QB - 1 - (qw * 32 + r));
+      if (j0 < wk.all_lo || j0 + 32 > wk.all_hi) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = j0 + 8 * (e >> 2) + 4 * h + (e & 3);
+          if (j < mine.lo || j >= mine.hi) s[e] = -INFINITY;
+        }
+      }
+      constexpr bool RAW = !CAP && BIAS == kBiasNone;  // still to be multiplied by scale2
+      float most = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
+      most = other_half(most, true);
+      if (RAW) most *= sc.scale2;
+      if (__any(most > top + kSlack)) {
+        const bool grow = most > top + kSlack;
+        const float old = grow ? __builtin_amdgcn_exp2f(top - most) : 1.0f;
+        top = grow ? most : top;
+        base = grow ? most - kLift : base;
+        sum *= old;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] *= old;
+      }
+      half8 p[2];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(RAW ? fmaf(s[e], sc.scale2, -base) : s[e] - base);
+        const float p1 =
+            __builtin_amdgcn_exp2f(RAW ? fmaf(s[e + 1], sc.scale2, -base) : s[e + 1] - base);
+        // fp16 probabilities for the product with V (they add 2^-12 of the output's own rounding,
+        // 2^-11, in the mean); the sum is that of the rounded ones, in fp32
+        const half2v two = __builtin_convertvector((float2v){p0, p1}, half2v);
+        p[e >> 3][e & 7] = two.x;
+        p[e >> 3][(e & 7) + 1] = two.y;
+        sum = __builtin_amdgcn_fdot2(two, half2v{1, 1}, sum, false);
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const int vrow = kb + 16 * st + 4 * h + ((lane & 15) >> 2);
+        const int ch = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          const half4 v0 = read_transposed(vt + vrow * DP + 32 * (dt ^ v_unit<DP>(vrow)) + ch);
+          const half4 v1 =
+              read_transposed(vt + (vrow + 8) * DP + 32 * (dt ^ v_unit<DP>(vrow + 8)) + ch);
+          const half8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[st], o[dt], 0, 0, 0);
+        }
+      }
+    }
+    if (tile + 1 < last) stage(buffer ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) product_done(o[dt]);
+  sum = other_half(sum, false);
+
+  if constexpr (KS > 1) {
+    // groups 1 .. KS - 1 hand over their sums; group 0 adds them in that order
+    constexpr int N = NDT * 16 + 2;
+    static_assert((KS - 1) * QW * N * 64 * 4 <= T::BYTES, "sums fit the tiles' LDS");
+    float* const box = reinterpret_cast<float*>(lds);
+    if (group > 0) {
+      float* const to = box + ((group - 1) * QW + qw) * N * 64 + lane;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) to[(16 * dt + e) * 64] = o[dt][e];
+      to[(N - 2) * 64] = top;
+      to[(N - 1) * 64] = sum;
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < KS; ++g) {
+      const float* const from = box + ((g - 1) * QW + qw) * N * 64 + lane;
+      const float top1 = from[(N - 2) * 64], both = fmaxf(top, top1);
+      const float c0 = top == both ? 1.0f : __builtin_amdgcn_exp2f(top - both);
+      const float c1 = top1 == both ? 1.0f : __builtin_amdgcn_exp2f(top1 - both);
+      sum = sum * c0 + from[(N - 1) * 64] * c1;
+      top = both;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * c0 + from[(16 * dt + e) * 64] * c1;
+    }
+  }
+
+  // A product of a probability of zero with a value that is not finite leaves NaN in a row that does
+  // not attend that value: rows that are not finite are computed again, each on its own.
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float odd = sum * 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd += o[dt][e] * 0.0f;
+  const unsigned long long found = __ballot(row && !(odd == 0.0f));
+  uint32_t again = static_cast<uint32_t>(found) | static_cast<uint32_t>(found >> 32);
+  if (row && !((again >> r) & 1)) {
+    _Float16* const out = static_cast<_Float16*>(a.out) + ((token + i) * a.H + head) * a.D;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int ch = 32 * dt + 8 * c + 4 * h;
+        if (ch < a.D)
+          *reinterpret_cast<half4*>(out + ch) =
+              half4{static_cast<_Float16>(o[dt][4 * c] * inv), static_cast<_Float16>(o[dt][4 * c + 1] * inv),
+                    static_cast<_Float16>(o[dt][4 * c + 2] * inv), static_cast<_Float16>(o[dt][4 * c + 3] * inv)};
+      }
+  }
+  while (again) {
+    const int n = __ffs(again) - 1;
+    again &= again - 1;
+    masked_row<_Float16>(a, b, i0 + qw * 32 + n, head, lane);
+  }
+}
+
+template <int DP, int KS>
+hipError_t launch_f16(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
+  constexpr int QB = 32 * (4 / KS);
+  const dim3 grid(static_cast<unsigned>(static_cast<uint64_t>(a.B) * a.H * ((a.S + QB - 1) / QB)));
+#define TESSERY_MASKED(CAP)                                                                  \
+  switch (a.bias_kind) {                                                                     \
+    case kBiasNone: attn_masked_f16<DP, KS, CAP, kBiasNone><<<grid, 256, 0, st>>>(a, s); break;     \
+    case kBiasSlopes: attn_masked_f16<DP, KS, CAP, kBiasSlopes><<<grid, 256, 0, st>>>(a, s); break; \
+    default: attn_masked_f16<DP, KS, CAP, kBiasTable><<<grid, 256, 0, st>>>(a, s); break;           \
+  }
+  if (a.cap > 0.0f) {
+    TESSERY_MASKED(true)
+  } else {
+    TESSERY_MASKED(false)
+  }
+#undef TESSERY_MASKED
+  return hipGetLastError();
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void attn_masked_rows(MaskedArgs a) {
   const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
@@ -113,10 +477,18 @@ bool attention_masked_fits(uint64_t B, uint64_t S, uint64_t H, uint64_t D) {
 hipError_t launch_attention_masked(const MaskedArgs& a, hipStream_t st) {
   const uint64_t rows = static_cast<uint64_t>(a.B) * a.S * a.H;
   const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
-  if (a.f16)
-    attn_masked_rows<_Float16><<<grid, 256, 0, st>>>(a);
-  else
-    attn_masked_rows<float><<<grid, 256, 0, st>>>(a);
+  if (a.f16) {
+    const float size = fabsf(a.scale) * kLog2e;
+    ScoreArgs s{};
+    s.q_sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
+    s.scale2 = a.cap > 0.0f ? 2.0f * size / a.cap : a.scale == 0.0f ? 1.0f : size;
+    s.cap2 = a.cap * kLog2e;
+    if (a.D <= 32) return launch_f16<32, 1>(a, s, st);
+    if (a.D <= 64) return launch_f16<64, 1>(a, s, st);
+    if (a.D <= 128) return launch_f16<128, 1>(a, s, st);
+    return launch_f16<256, 1>(a, s, st);
+  }
+  attn_masked_rows<float><<<grid, 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
