@@ -10,6 +10,9 @@
 #include "kernels.h"
 
 #include <math.h>
+#include <stdlib.h>
+
+#include <type_traits>
 
 namespace tessery {
 namespace {
@@ -173,6 +176,176 @@ __device__ __forceinline__ void score_block(floatx16& v, const ScoreArgs& s, flo
   }
 }
 
+// Where a workgroup of four wavefronts works: 4 / KS wavefronts of 32 queries of one head each, in KS
+// groups that share the keys out. Lane l holds query r = l % 32, as its half h = l / 32.
+template <int KS>
+struct Place {
+  static constexpr int QW = 4 / KS, QB = 32 * QW;
+  int lane, r, h, wave, qw, group, head, kvh, b, i0, i, L;
+  size_t token;
+  bool row;        // i is a query
+  KeyRange mine;   // the keys of query i
+  WaveKeys keys;
+
+  __device__ __forceinline__ Place(const MaskedArgs& a, int (*ends)[2]) {
+    lane = threadIdx.x & 63;
+    r = lane & 31;
+    h = lane >> 5;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    qw = wave % QW;
+    group = wave / QW;
+    const int blocks = (a.S + QB - 1) / QB;
+    int at = static_cast<int>(blockIdx.x);
+    const int qb = blocks - 1 - at % blocks;  // the last (causally longest) blocks of a head first
+    at /= blocks;
+    head = at % a.H;
+    b = at / a.H;
+    kvh = head / (a.H / a.KV);
+    i0 = qb * QB;
+    i = i0 + qw * 32 + r;
+    row = i < a.S;
+    mine = key_range(a, b, min(i, a.S - 1));
+    keys = wave_keys(mine, row);
+    if (lane == 0) {
+      ends[wave][0] = keys.lo;
+      ends[wave][1] = keys.hi;
+    }
+    L = static_cast<int>(min(a.lengths[b], static_cast<uint32_t>(a.S)));
+    token = static_cast<size_t>(b) * a.S;
+  }
+
+  // the tiles of `size` keys that the workgroup walks; none where nothing is attended
+  __device__ __forceinline__ void tiles(const int (*ends)[2], int size, int* first, int* last) const {
+    __syncthreads();
+    int lo = ends[0][0], hi = ends[0][1];
+#pragma unroll
+    for (int n = 1; n < QW; ++n) {
+      lo = min(lo, ends[n][0]);
+      hi = max(hi, ends[n][1]);
+    }
+    *first = lo / size;
+    *last = (hi + size - 1) / size;
+  }
+
+  // whether no row of this wavefront attends a key of the block of 32 from j0, and whether some row does
+  // not attend them all
+  __device__ __forceinline__ bool skips(int j0) const { return j0 >= keys.hi || j0 + 32 <= keys.lo; }
+  __device__ __forceinline__ bool partial(int j0) const {
+    return j0 < keys.all_lo || j0 + 32 > keys.all_hi;
+  }
+  __device__ __forceinline__ void mask(floatx16& s, int j0) const {
+    if (!partial(j0)) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int j = j0 + 8 * (e >> 2) + 4 * h + (e & 3);
+      if (j < mine.lo || j >= mine.hi) s[e] = -INFINITY;
+    }
+  }
+};
+
+// The online softmax of one query: the running maximum (in log2 units), what exponents are taken less
+// of, and this lane's share of the sum.
+template <int NDT>
+struct Softmax {
+  float top = -INFINITY, base = 0.0f, sum = 0.0f;
+  floatx16 o[NDT];
+
+  __device__ __forceinline__ Softmax() {
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+  }
+
+  // takes in the block's largest score, `factor` times that of s
+  __device__ __forceinline__ void raise(const floatx16& s, float factor, float lift) {
+    float most = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
+    most = other_half(most, true) * factor;
+    const bool grow = most > top + kSlack;
+    if (__any(grow)) {
+      const float old = grow ? __builtin_amdgcn_exp2f(top - most) : 1.0f;
+      top = grow ? most : top;
+      base = grow ? most - lift : base;
+      sum *= old;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o[dt] *= old;
+    }
+  }
+
+  // After the last tile: the lanes' shares of the sum meet, then the groups' results: groups
+  // 1 .. KS - 1 hand theirs over in `box` and group 0 adds them in that order. False: not group 0.
+  static constexpr int BOX = NDT * 16 + 2;
+  template <int KS>
+  __device__ __forceinline__ bool join(const Place<KS>& w, float* box) {
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) product_done(o[dt]);
+    sum = other_half(sum, false);
+    if constexpr (KS > 1) {
+      if (w.group > 0) {
+        float* const to = box + ((w.group - 1) * w.QW + w.qw) * BOX * 64 + w.lane;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) to[(16 * dt + e) * 64] = o[dt][e];
+        to[(BOX - 2) * 64] = top;
+        to[(BOX - 1) * 64] = sum;
+      }
+      __syncthreads();
+      if (w.group > 0) return false;
+#pragma unroll
+      for (int g = 1; g < KS; ++g) {
+        const float* const from = box + ((g - 1) * w.QW + w.qw) * BOX * 64 + w.lane;
+        const float top1 = from[(BOX - 2) * 64], both = fmaxf(top, top1);
+        const float c0 = top == both ? 1.0f : __builtin_amdgcn_exp2f(top - both);
+        const float c1 = top1 == both ? 1.0f : __builtin_amdgcn_exp2f(top1 - both);
+        sum = sum * c0 + from[(BOX - 1) * 64] * c1;
+        top = both;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * c0 + from[(16 * dt + e) * 64] * c1;
+      }
+    }
+    return true;
+  }
+
+  // Stores the wavefront's rows. A product of a probability of zero with a value that is not finite
+  // leaves NaN in a row that does not attend that value: rows that are not finite are computed again,
+  // each on its own.
+  template <typename T, int KS>
+  __device__ __forceinline__ void store(const MaskedArgs& a, const Place<KS>& w) const {
+    typedef T out4 __attribute__((ext_vector_type(4)));
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float odd = sum * 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) odd += o[dt][e] * 0.0f;
+    const unsigned long long found = __ballot(w.row && !(odd == 0.0f));
+    uint32_t again = static_cast<uint32_t>(found) | static_cast<uint32_t>(found >> 32);
+    if (w.row && !((again >> w.r) & 1)) {
+      T* const out = static_cast<T*>(a.out) + ((w.token + w.i) * a.H + w.head) * a.D;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int ch = 32 * dt + 8 * c + 4 * w.h;
+          if (ch < a.D)
+            *reinterpret_cast<out4*>(out + ch) =
+                out4{static_cast<T>(o[dt][4 * c] * inv), static_cast<T>(o[dt][4 * c + 1] * inv),
+                     static_cast<T>(o[dt][4 * c + 2] * inv), static_cast<T>(o[dt][4 * c + 3] * inv)};
+        }
+    }
+    while (again) {
+      const int n = __ffs(again) - 1;
+      again &= again - 1;
+      masked_row<T>(a, w.b, w.i0 + w.qw * 32 + n, w.head, w.lane);
+    }
+  }
+};
+
 // Tiles of fp16 operands on v_mfma_f32_32x32x16_f16: lane (r = l % 32, h = l / 32) supplies A[r][8h ..
 // 8h + 7] and B[8h .. 8h + 7][r] and holds D[8a + 4h + c][r] in element 4a + c.
 //   S^T = K Q^T for blocks of 32 keys x 32 queries: a query's scores lie in the two lanes r and r + 32.
@@ -201,7 +374,7 @@ __device__ __forceinline__ int v_unit(int row) {
 template <int DP, int KS, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(MaskedArgs a, ScoreArgs sc) {
   using T = F16Tile<DP>;
-  constexpr int KT = T::KT, QW = 4 / KS, QB = 32 * QW, NS = DP / 16, NDT = DP / 32;
+  constexpr int KT = T::KT, QB = 128 / KS, NS = DP / 16, NDT = DP / 32;
   constexpr int NB = KT / 32 / KS;  // key blocks of a tile that one wavefront takes
   static_assert(NB >= 1, "a block of keys for every group");
   __shared__ __attribute__((aligned(16))) char lds[T::BYTES];
@@ -210,27 +383,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(Masked
   _Float16* const vt0 = kt0 + 2 * T::K;
   float* const bt0 = reinterpret_cast<float*>(vt0 + 2 * T::V);
 
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int qw = wave % QW, group = wave / QW;
-  const int blocks = (a.S + QB - 1) / QB;
-  // the last (causally longest) blocks of a head first
-  int at = static_cast<int>(blockIdx.x);
-  const int qb = blocks - 1 - at % blocks;
-  at /= blocks;
-  const int head = at % a.H, b = at / a.H;
-  const int kvh = head / (a.H / a.KV);
-  const int i0 = qb * QB, i = i0 + qw * 32 + r;
-  const bool row = i < a.S;
+  const Place<KS> w(a, ends);
+  const int tid = threadIdx.x, lane = w.lane, r = w.r, h = w.h, i = w.i;
+  const int b = w.b, head = w.head, kvh = w.kvh, L = w.L;
+  const size_t token = w.token;
   const int ic = min(i, a.S - 1);
-  const KeyRange mine = key_range(a, b, ic);
-  const WaveKeys wk = wave_keys(mine, row);
-  if (lane == 0) {
-    ends[wave][0] = wk.lo;
-    ends[wave][1] = wk.hi;
-  }
-  const int L = static_cast<int>(min(a.lengths[b], static_cast<uint32_t>(a.S)));
-  const size_t token = static_cast<size_t>(b) * a.S;
   const _Float16* const q = static_cast<const _Float16*>(a.q) + (token + ic) * a.q_row + head * a.D;
   const _Float16* const k = static_cast<const _Float16*>(a.k) + token * a.k_row + kvh * a.D;
   const _Float16* const v = static_cast<const _Float16*>(a.v) + token * a.v_row + kvh * a.D;
@@ -247,14 +404,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(Masked
   const float slope2 = BIAS == kBiasSlopes ? a.bias[head] * kLog2e : 0.0f;
   const float* const table =
       BIAS == kBiasTable ? a.bias + head * (2 * static_cast<size_t>(a.radius) + 1) : nullptr;
-  __syncthreads();
-  int lo = ends[0][0], hi = ends[0][1];
-#pragma unroll
-  for (int w = 1; w < QW; ++w) {
-    lo = min(lo, ends[w][0]);
-    hi = max(hi, ends[w][1]);
-  }
-  const int first = lo / KT, last = (hi + KT - 1) / KT;  // hi 0: no tile
+  int first, last;
+  w.tiles(ends, KT, &first, &last);
 
   // staging: thread t takes 16-byte pieces t, t + 256, ... of the tile
   half8 kreg[T::CHUNKS], vreg[T::CHUNKS];
@@ -271,7 +422,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(Masked
     }
     if constexpr (BIAS == kBiasTable) {
       // entry x: distance key - query of tile * KT - i0 + x - (QB - 1)
-      const int away = tile * KT - i0 + tid - (QB - 1);
+      const int away = tile * KT - w.i0 + tid - (QB - 1);
       if (tid < KT + QB - 1) breg = log2_bias(table[min(max(away, -a.radius), a.radius) + a.radius]);
     }
   };
@@ -288,13 +439,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(Masked
       if (tid < KT + QB - 1) bt0[buffer * T::BIASES + tid] = breg;
   };
 
-  floatx16 o[NDT];
-#pragma unroll
-  for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-  float top = -INFINITY, base = 0.0f, sum = 0.0f;
-
+  Softmax<NDT> soft;
   if (first < last) {
     fetch(first);
     stage(0);
@@ -307,8 +452,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(Masked
     const _Float16* const vt = vt0 + buffer * T::V;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int kb = (KS == 1 ? nb : group) * 32, j0 = tile * KT + kb;
-      if (j0 >= wk.hi || j0 + 32 <= wk.lo) continue;  // wavefront-uniform
+      const int kb = (KS == 1 ? nb : w.group) * 32, j0 = tile * KT + kb;
+      if (w.skips(j0)) continue;  // wavefront-uniform
       floatx16 s;
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 0.0f;
@@ -319,41 +464,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(Masked
       }
       product_done(s);
       score_block<CAP, BIAS>(s, sc, slope2, static_cast<float>(j0 + 4 * h - i),
-                             bt0 + buffer * T::BIASES + kb + 4 * h + QB - 1 - (qw * 32 + r));
-      if (j0 < wk.all_lo || j0 + 32 > wk.all_hi) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int j = j0 + 8 * (e >> 2) + 4 * h + (e & 3);
-          if (j < mine.lo || j >= mine.hi) s[e] = -INFINITY;
-        }
-      }
+                             bt0 + buffer * T::BIASES + kb + 4 * h + QB - 1 - (w.qw * 32 + r));
+      w.mask(s, j0);
       constexpr bool RAW = !CAP && BIAS == kBiasNone;  // still to be multiplied by scale2
-      float most = s[0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
-      most = other_half(most, true);
-      if (RAW) most *= sc.scale2;
-      if (__any(most > top + kSlack)) {
-        const bool grow = most > top + kSlack;
-        const float old = grow ? __builtin_amdgcn_exp2f(top - most) : 1.0f;
-        top = grow ? most : top;
-        base = grow ? most - kLift : base;
-        sum *= old;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[dt] *= old;
-      }
+      soft.raise(s, RAW ? sc.scale2 : 1.0f, kLift);
       half8 p[2];
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(RAW ? fmaf(s[e], sc.scale2, -base) : s[e] - base);
+        const float p0 = __builtin_amdgcn_exp2f(RAW ? fmaf(s[e], sc.scale2, -soft.base) : s[e] - soft.base);
         const float p1 =
-            __builtin_amdgcn_exp2f(RAW ? fmaf(s[e + 1], sc.scale2, -base) : s[e + 1] - base);
+            __builtin_amdgcn_exp2f(RAW ? fmaf(s[e + 1], sc.scale2, -soft.base) : s[e + 1] - soft.base);
         // fp16 probabilities for the product with V (they add 2^-12 of the output's own rounding,
         // 2^-11, in the mean); the sum is that of the rounded ones, in fp32
         const half2v two = __builtin_convertvector((float2v){p0, p1}, half2v);
         p[e >> 3][e & 7] = two.x;
         p[e >> 3][(e & 7) + 1] = two.y;
-        sum = __builtin_amdgcn_fdot2(two, half2v{1, 1}, sum, false);
+        soft.sum = __builtin_amdgcn_fdot2(two, half2v{1, 1}, soft.sum, false);
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
@@ -365,106 +491,191 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(Masked
           const half4 v1 =
               read_transposed(vt + (vrow + 8) * DP + 32 * (dt ^ v_unit<DP>(vrow + 8)) + ch);
           const half8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[st], o[dt], 0, 0, 0);
+          soft.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[st], soft.o[dt], 0, 0, 0);
         }
       }
     }
     if (tile + 1 < last) stage(buffer ^ 1);
     __syncthreads();
   }
-#pragma unroll
-  for (int dt = 0; dt < NDT; ++dt) product_done(o[dt]);
-  sum = other_half(sum, false);
-
-  if constexpr (KS > 1) {
-    // groups 1 .. KS - 1 hand over their sums; group 0 adds them in that order
-    constexpr int N = NDT * 16 + 2;
-    static_assert((KS - 1) * QW * N * 64 * 4 <= T::BYTES, "sums fit the tiles' LDS");
-    float* const box = reinterpret_cast<float*>(lds);
-    if (group > 0) {
-      float* const to = box + ((group - 1) * QW + qw) * N * 64 + lane;
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) to[(16 * dt + e) * 64] = o[dt][e];
-      to[(N - 2) * 64] = top;
-      to[(N - 1) * 64] = sum;
-    }
-    __syncthreads();
-    if (group > 0) return;
-#pragma unroll
-    for (int g = 1; g < KS; ++g) {
-      const float* const from = box + ((g - 1) * QW + qw) * N * 64 + lane;
-      const float top1 = from[(N - 2) * 64], both = fmaxf(top, top1);
-      const float c0 = top == both ? 1.0f : __builtin_amdgcn_exp2f(top - both);
-      const float c1 = top1 == both ? 1.0f : __builtin_amdgcn_exp2f(top1 - both);
-      sum = sum * c0 + from[(N - 1) * 64] * c1;
-      top = both;
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * c0 + from[(16 * dt + e) * 64] * c1;
-    }
-  }
-
-  // A product of a probability of zero with a value that is not finite leaves NaN in a row that does
-  // not attend that value: rows that are not finite are computed again, each on its own.
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  float odd = sum * 0.0f;
-#pragma unroll
-  for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) odd += o[dt][e] * 0.0f;
-  const unsigned long long found = __ballot(row && !(odd == 0.0f));
-  uint32_t again = static_cast<uint32_t>(found) | static_cast<uint32_t>(found >> 32);
-  if (row && !((again >> r) & 1)) {
-    _Float16* const out = static_cast<_Float16*>(a.out) + ((token + i) * a.H + head) * a.D;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int ch = 32 * dt + 8 * c + 4 * h;
-        if (ch < a.D)
-          *reinterpret_cast<half4*>(out + ch) =
-              half4{static_cast<_Float16>(o[dt][4 * c] * inv), static_cast<_Float16>(o[dt][4 * c + 1] * inv),
-                    static_cast<_Float16>(o[dt][4 * c + 2] * inv), static_cast<_Float16>(o[dt][4 * c + 3] * inv)};
-      }
-  }
-  while (again) {
-    const int n = __ffs(again) - 1;
-    again &= again - 1;
-    masked_row<_Float16>(a, b, i0 + qw * 32 + n, head, lane);
-  }
+  static_assert((KS - 1) * (4 / KS) * Softmax<NDT>::BOX * 256 <= T::BYTES, "sums fit the tiles' LDS");
+  if (soft.join(w, reinterpret_cast<float*>(lds))) soft.template store<_Float16>(a, w);
 }
 
-template <int DP, int KS>
-hipError_t launch_f16(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
-  constexpr int QB = 32 * (4 / KS);
+// Tiles of fp32 operands on v_mfma_f32_32x32x2_f32: lane (r, h) supplies A[r][h] and B[h][r], D as above.
+//   S^T = K Q^T: step s takes channels s and s + DP / 2, so that a lane's values of Q are neighbours.
+//   O^T = V^T P^T: the two keys of step e are those of the lanes' element e. A row of V lies in LDS with its
+//   32-channel blocks interleaved, so one read gives a lane its channel of every block.
+// Everything is fp32: products, sums, probabilities.
+template <int DP>
+struct F32Tile {
+  static constexpr int KT = DP >= 128 ? 32 : 64;
+  static constexpr int KROW = DP + 4;
+  static constexpr int K = KT * KROW, V = KT * DP;
+  static constexpr int CHUNKS = KT * DP / 4 / 256;
+  static constexpr int BIASES = 192;
+  static constexpr int BYTES = (2 * (K + V) + 2 * BIASES) * 4;
+};
+
+template <int DP, int KS, bool CAP, int BIAS>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f32(MaskedArgs a, ScoreArgs sc) {
+  using T = F32Tile<DP>;
+  constexpr int KT = T::KT, QB = 128 / KS, NDT = DP / 32, HALF = DP / 2;
+  constexpr int NB = KT / 32 / KS;  // key blocks of a tile that one wavefront takes
+  static_assert(NB >= 1, "a block of keys for every group");
+  __shared__ __attribute__((aligned(16))) char lds[T::BYTES];
+  __shared__ int ends[4][2];
+  float* const kt0 = reinterpret_cast<float*>(lds);
+  float* const vt0 = kt0 + 2 * T::K;
+  float* const bt0 = vt0 + 2 * T::V;
+
+  const Place<KS> w(a, ends);
+  const int tid = threadIdx.x, r = w.r, h = w.h;
+  const int ic = min(w.i, a.S - 1);
+  const float* const q = static_cast<const float*>(a.q) + (w.token + ic) * a.q_row + w.head * a.D;
+  const float* const k = static_cast<const float*>(a.k) + w.token * a.k_row + w.kvh * a.D;
+  const float* const v = static_cast<const float*>(a.v) + w.token * a.v_row + w.kvh * a.D;
+  floatx4 qf[HALF / 4];
+#pragma unroll
+  for (int c = 0; c < HALF / 4; ++c) {
+    const int ch = h * HALF + 4 * c;
+    qf[c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (ch < a.D) qf[c] = *reinterpret_cast<const floatx4*>(q + ch) * sc.q_sign;
+  }
+  const float slope2 = BIAS == kBiasSlopes ? a.bias[w.head] * kLog2e : 0.0f;
+  const float* const table =
+      BIAS == kBiasTable ? a.bias + w.head * (2 * static_cast<size_t>(a.radius) + 1) : nullptr;
+  int first, last;
+  w.tiles(ends, KT, &first, &last);
+
+  floatx4 kreg[T::CHUNKS], vreg[T::CHUNKS];
+  float breg = 0.0f;
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int c = 0; c < T::CHUNKS; ++c) {
+      const int piece = tid + 256 * c, key = tile * KT + piece / (DP / 4), ch = piece % (DP / 4) * 4;
+      kreg[c] = vreg[c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (key < w.L && ch < a.D) {
+        kreg[c] = *reinterpret_cast<const floatx4*>(k + static_cast<size_t>(key) * a.k_row + ch);
+        vreg[c] = *reinterpret_cast<const floatx4*>(v + static_cast<size_t>(key) * a.v_row + ch);
+      }
+    }
+    if constexpr (BIAS == kBiasTable) {
+      const int away = tile * KT - w.i0 + tid - (QB - 1);
+      if (tid < KT + QB - 1) breg = log2_bias(table[min(max(away, -a.radius), a.radius) + a.radius]);
+    }
+  };
+  auto stage = [&](int buffer) {
+    float* const kt = kt0 + buffer * T::K;
+    float* const vt = vt0 + buffer * T::V;
+#pragma unroll
+    for (int c = 0; c < T::CHUNKS; ++c) {
+      const int piece = tid + 256 * c, key = piece / (DP / 4), ch = piece % (DP / 4) * 4;
+      *reinterpret_cast<floatx4*>(kt + key * T::KROW + ch) = kreg[c];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        vt[key * DP + ((ch + j) & 31) * NDT + ((ch + j) >> 5)] = vreg[c][j];
+    }
+    if constexpr (BIAS == kBiasTable)
+      if (tid < KT + QB - 1) bt0[buffer * T::BIASES + tid] = breg;
+  };
+
+  Softmax<NDT> soft;
+  if (first < last) {
+    fetch(first);
+    stage(0);
+  }
+  __syncthreads();
+  for (int tile = first; tile < last; ++tile) {
+    const int buffer = (tile - first) & 1;
+    if (tile + 1 < last) fetch(tile + 1);
+    const float* const kt = kt0 + buffer * T::K;
+    const float* const vt = vt0 + buffer * T::V;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int kb = (KS == 1 ? nb : w.group) * 32, j0 = tile * KT + kb;
+      if (w.skips(j0)) continue;  // wavefront-uniform
+      floatx16 s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < HALF / 4; ++c) {
+        const floatx4 kf = *reinterpret_cast<const floatx4*>(kt + (kb + r) * T::KROW + h * HALF + 4 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[c][j], s, 0, 0, 0);
+      }
+      product_done(s);
+      score_block<CAP, BIAS>(s, sc, slope2, static_cast<float>(j0 + 4 * h - w.i),
+                             bt0 + buffer * T::BIASES + kb + 4 * h + QB - 1 - (w.qw * 32 + r));
+      w.mask(s, j0);
+      constexpr bool RAW = !CAP && BIAS == kBiasNone;
+      soft.raise(s, RAW ? sc.scale2 : 1.0f, 0.0f);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(RAW ? fmaf(s[e], sc.scale2, -soft.base) : s[e] - soft.base);
+        soft.sum += s[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float* const vr = vt + (kb + 8 * (e >> 2) + 4 * h + (e & 3)) * DP + r * NDT;
+        float vf[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) vf[dt] = vr[dt];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+          soft.o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[dt], s[e], soft.o[dt], 0, 0, 0);
+      }
+    }
+    if (tile + 1 < last) stage(buffer ^ 1);
+    __syncthreads();
+  }
+  static_assert((KS - 1) * (4 / KS) * Softmax<NDT>::BOX * 256 <= T::BYTES, "sums fit the tiles' LDS");
+  if (soft.join(w, reinterpret_cast<float*>(lds))) soft.template store<float>(a, w);
+}
+
+// f(CAP, BIAS) as compile-time values
+template <typename F>
+void for_scores(const MaskedArgs& a, F&& f) {
+  using None = std::integral_constant<int, kBiasNone>;
+  using Slopes = std::integral_constant<int, kBiasSlopes>;
+  using Table = std::integral_constant<int, kBiasTable>;
+  auto with = [&](auto cap) {
+    if (a.bias_kind == kBiasNone) f(cap, None{});
+    else if (a.bias_kind == kBiasSlopes) f(cap, Slopes{});
+    else f(cap, Table{});
+  };
+  if (a.cap > 0.0f) with(std::true_type{});
+  else with(std::false_type{});
+}
+
+template <bool F16, int DP, int KS>
+hipError_t launch_tiles(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
+  constexpr int QB = 128 / KS;
   const dim3 grid(static_cast<unsigned>(static_cast<uint64_t>(a.B) * a.H * ((a.S + QB - 1) / QB)));
-#define TESSERY_MASKED(CAP)                                                                  \
-  switch (a.bias_kind) {                                                                     \
-    case kBiasNone: attn_masked_f16<DP, KS, CAP, kBiasNone><<<grid, 256, 0, st>>>(a, s); break;     \
-    case kBiasSlopes: attn_masked_f16<DP, KS, CAP, kBiasSlopes><<<grid, 256, 0, st>>>(a, s); break; \
-    default: attn_masked_f16<DP, KS, CAP, kBiasTable><<<grid, 256, 0, st>>>(a, s); break;           \
-  }
-  if (a.cap > 0.0f) {
-    TESSERY_MASKED(true)
-  } else {
-    TESSERY_MASKED(false)
-  }
-#undef TESSERY_MASKED
+  for_scores(a, [&](auto cap, auto bias) {
+    if constexpr (F16)
+      attn_masked_f16<DP, KS, decltype(cap)::value, decltype(bias)::value><<<grid, 256, 0, st>>>(a, s);
+    else
+      attn_masked_f32<DP, KS, decltype(cap)::value, decltype(bias)::value><<<grid, 256, 0, st>>>(a, s);
+  });
   return hipGetLastError();
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void attn_masked_rows(MaskedArgs a) {
-  const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const uint64_t per = static_cast<uint64_t>(a.S) * a.H;
-  if (row >= a.B * per) return;  // wavefront-uniform
-  const int b = static_cast<int>(row / per);
-  const uint32_t rest = static_cast<uint32_t>(row - b * per);
-  masked_row<T>(a, b, static_cast<int>(rest / a.H), static_cast<int>(rest % a.H),
-                threadIdx.x & 63);
+template <bool F16, int DP>
+hipError_t launch_split(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
+  static const int ks = getenv("TESSERY_KS") ? atoi(getenv("TESSERY_KS")) : 1;
+  if constexpr (DP <= (F16 ? 128 : 64))
+    if (ks == 2) return launch_tiles<F16, DP, 2>(a, s, st);
+  return launch_tiles<F16, DP, 1>(a, s, st);
+}
+
+template <bool F16>
+hipError_t launch_sized(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
+  if (a.D <= 32) return launch_split<F16, 32>(a, s, st);
+  if (a.D <= 64) return launch_split<F16, 64>(a, s, st);
+  if (a.D <= 128) return launch_split<F16, 128>(a, s, st);
+  return launch_split<F16, 256>(a, s, st);
 }
 
 }  // namespace
@@ -475,21 +686,12 @@ bool attention_masked_fits(uint64_t B, uint64_t S, uint64_t H, uint64_t D) {
 }
 
 hipError_t launch_attention_masked(const MaskedArgs& a, hipStream_t st) {
-  const uint64_t rows = static_cast<uint64_t>(a.B) * a.S * a.H;
-  const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
-  if (a.f16) {
-    const float size = fabsf(a.scale) * kLog2e;
-    ScoreArgs s{};
-    s.q_sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
-    s.scale2 = a.cap > 0.0f ? 2.0f * size / a.cap : a.scale == 0.0f ? 1.0f : size;
-    s.cap2 = a.cap * kLog2e;
-    if (a.D <= 32) return launch_f16<32, 1>(a, s, st);
-    if (a.D <= 64) return launch_f16<64, 1>(a, s, st);
-    if (a.D <= 128) return launch_f16<128, 1>(a, s, st);
-    return launch_f16<256, 1>(a, s, st);
-  }
-  attn_masked_rows<float><<<grid, 256, 0, st>>>(a);
-  return hipGetLastError();
+  const float size = fabsf(a.scale) * kLog2e;
+  ScoreArgs s{};
+  s.q_sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
+  s.scale2 = a.cap > 0.0f ? 2.0f * size / a.cap : a.scale == 0.0f ? 1.0f : size;
+  s.cap2 = a.cap * kLog2e;
+  return a.f16 ? launch_sized<true>(a, s, st) : launch_sized<false>(a, s, st);
 }
 
 }  // namespace tessery
