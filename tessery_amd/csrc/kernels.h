@@ -296,8 +296,6 @@ struct LinearF16Args {
   const _Float16* residual;
   void* out;
   int M, N, K, act, out_f32;
-  float* scratch;  // partial sums
-  size_t scratch_floats;
 };
 hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st);
 

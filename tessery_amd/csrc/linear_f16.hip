@@ -5,33 +5,54 @@
 // residual are applied to the fp32 sum and one rounding to the output's type ends it.
 #include "common.h"
 #include "kernels.h"
+#include "lds_dma.h"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace tessery {
 namespace {
 
-__device__ __forceinline__ float activate(float y, int act) {
-  switch (act) {
-    case kActRelu:
-      return y < 0.0f ? 0.0f : y;
-    case kActGelu:
-      return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
-    case kActGeluTanh:  // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3)
-      return y / (1.0f + expf(-1.5957691216057308f * fmaf(0.044715f * y * y, y, y)));
-    case kActSilu:
-      return y / (1.0f + expf(-y));
-    default:
-      return y;
-  }
+// 1 / (1 + 2^-x)
+__device__ __forceinline__ float logistic(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x));
+}
+
+// y times the normal distribution's integral up to y, y (1 + erf(y / sqrt 2)) / 2, as max(y, 0) - t P(-t)
+// with t = |y|. The integral up to -t is exp(-t^2 / 2) times a polynomial in u = 1 / (1 + p t) (the form of
+// Abramowitz and Stegun 7.1.26; p and the coefficients are a weighted minimax fit to the function, off by
+// less than 1e-8, 2e-7 with fp32 rounding). erff took 56 us of a 16384 x 4096 output, this 32 us.
+__device__ __forceinline__ float gelu(float y) {
+  const float t = fabsf(y), u = __builtin_amdgcn_rcpf(fmaf(0.28f, t, 1.0f));
+  float s = -0.10580878214302342f;
+  s = fmaf(s, u, 0.3898762044949095f);
+  s = fmaf(s, u, -0.23699701042804464f);
+  s = fmaf(s, u, 0.26891299545827674f);
+  s = fmaf(s, u, 0.06749562607910956f);
+  s = fmaf(s, u, 0.11652095725613074f);
+  const float below = s * u * __builtin_amdgcn_exp2f(t * (t * -0.72134752044448170f));
+  return fmaf(-fminf(t, 1e18f), below, fmaxf(y, 0.0f));  // an infinite t times 0 would be NaN
+}
+
+template <int ACT>
+__device__ __forceinline__ float activate(float y) {
+  if constexpr (ACT == kActRelu) return y < 0.0f ? 0.0f : y;
+  if constexpr (ACT == kActGelu) return gelu(y);
+  // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3)
+  if constexpr (ACT == kActGeluTanh)
+    return y * logistic(1.5957691216057308f * kLog2e * fmaf(0.044715f * y * y, y, y));
+  if constexpr (ACT == kActSilu) return y * logistic(kLog2e * y);
+  return y;
 }
 
 // Four consecutive columns n .. n + 3 of row m.
+template <int ACT>
 __device__ __forceinline__ void finish4(const LinearF16Args& a, int m, int n, floatx4 y) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (n + j >= a.N) return;
-    float r = activate(y[j] + (a.bias ? a.bias[n + j] : 0.0f), a.act);
+    float r = activate<ACT>(y[j] + (a.bias ? a.bias[n + j] : 0.0f));
     const size_t at = static_cast<size_t>(m) * a.N + n + j;
     if (a.residual) r += static_cast<float>(a.residual[at]);
     if (a.out_f32)
@@ -45,24 +66,20 @@ __device__ __forceinline__ void finish4(const LinearF16Args& a, int m, int n, fl
 // g = l / 32) supplies A[r][8g..8g+7] and B[8g..8g+7][r] and holds D[8a + 4g + c][r] in element
 // 4a + c), 32 of K at a time through registers into LDS. A is W and B is x, so that a lane's four
 // elements are neighbours in a row of out. Any M, N and K.
-__global__ __launch_bounds__(256) void linear_f16_any(LinearF16Args a) {
+template <int ACT>
+__global__ __launch_bounds__(256) void linear_f16_any(LinearF16Args a, int tiles_n) {
   constexpr int KT = 32, ROW = KT + 8;
   __shared__ __attribute__((aligned(16))) _Float16 ws[64 * ROW], xs[64 * ROW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n0 = blockIdx.x * 64, m0 = blockIdx.y * 64;
+  const int n0 = static_cast<int>(blockIdx.x) % tiles_n * 64, m0 = static_cast<int>(blockIdx.x) / tiles_n * 64;
   const int lr = tid >> 2, lc = (tid & 3) * 8;
-  const bool whole = a.K % 8 == 0;
   auto fetch = [&](const _Float16* p, int row, int rows, int k) {
     half8 v = {};
     if (row < rows) {
       const _Float16* at = p + static_cast<size_t>(row) * a.K + k;
-      if (whole) {
-        if (k < a.K) v = *reinterpret_cast<const half8*>(at);
-      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k + j < a.K) v[j] = at[j];
-      }
+      for (int j = 0; j < 8; ++j)
+        if (k + j < a.K) v[j] = at[j];
     }
     return v;
   };
@@ -87,16 +104,392 @@ __global__ __launch_bounds__(256) void linear_f16_any(LinearF16Args a) {
   if (m >= a.M) return;
 #pragma unroll
   for (int q = 0; q < 4; ++q)
-    finish4(a, m, n0 + nw + 8 * q + 4 * g,
+    finish4<ACT>(a, m, n0 + nw + 8 * q + 4 * g,
             floatx4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]});
+}
+
+// TM x TN outputs a workgroup of WM x WN wavefronts, K taken BK at a time through a ring of NST stages in
+// LDS that global_load_lds_dwordx4 fills NST - 1 stages ahead. A row of a stage is BK halves; its 16-byte
+// chunks are XORed with sw(row), so the 16 rows of a read fall on 16 bank groups. Rows past M or N read the
+// last row and are not stored; the chunks of a last stage past K are left out as the operands are read.
+// Needs K % 8 == 0.
+template <int BK>
+__device__ __forceinline__ int sw(int row) {
+  static_assert(BK == 64 || BK == 128, "rows of a half or a whole line of banks");
+  return BK == 128 ? row & 15 : (row >> 1) & 7;
+}
+
+template <int TM, int TN, int WM, int WN, int BK, int NST>
+struct TileShape {
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int MB = TM / WM / 32, NB = TN / WN / 32;  // 32 x 32 blocks of a wavefront
+  static constexpr int CPR = BK / 8;                          // chunks of a row
+  static constexpr int STAGE = (TM + TN) * BK;                // halves
+  static constexpr int LOADS = STAGE / 512 / WAVES;           // 1 KiB blocks a wavefront fills
+  static constexpr int ROWS = 64 / CPR;                       // rows of a block
+  static constexpr int OUT = TN / WN + 4;                     // floats of a row staged for the stores
+  static constexpr int BYTES = NST * STAGE * 2 > WAVES * 32 * OUT * 4 ? NST * STAGE * 2 : WAVES * 32 * OUT * 4;
+  static_assert(STAGE % (512 * WAVES) == 0 && TM * BK % 512 == 0, "whole blocks");
+};
+
+// Eight columns n .. n + 7 of row m from fp32 sums that bias and activation have been applied to.
+__device__ __forceinline__ void store8(const LinearF16Args& a, int m, int n, const float* y) {
+  const size_t at = static_cast<size_t>(m) * a.N + n;
+  float r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = y[j];
+  if (a.N % 8 == 0) {
+    if (a.residual) {
+      const half8 v = *reinterpret_cast<const half8*>(a.residual + at);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] += static_cast<float>(v[j]);
+    }
+    if (a.out_f32) {
+      floatx4* const o = reinterpret_cast<floatx4*>(static_cast<float*>(a.out) + at);
+      o[0] = floatx4{r[0], r[1], r[2], r[3]};
+      o[1] = floatx4{r[4], r[5], r[6], r[7]};
+    } else {
+      half8 v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = static_cast<_Float16>(r[j]);
+      *reinterpret_cast<half8*>(static_cast<_Float16*>(a.out) + at) = v;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (n + j >= a.N) return;
+    if (a.residual) r[j] += static_cast<float>(a.residual[at + j]);
+    if (a.out_f32) static_cast<float*>(a.out)[at + j] = r[j];
+    else static_cast<_Float16*>(a.out)[at + j] = static_cast<_Float16>(r[j]);
+  }
+}
+
+// Workgroups go round the eight XCDs, each with an L2 of its own: an XCD takes a run of tiles, walked in
+// bands of kBand tiles of M, so that the tiles that run on it together share rows of x and of W.
+constexpr int kBand = 8;
+struct TilePlace {
+  int m, n;
+  __device__ __forceinline__ TilePlace(int tiles_m, int tiles_n) {
+    const int tiles = tiles_m * tiles_n, id = static_cast<int>(blockIdx.x);
+    const int xcd = id & 7, each = tiles >> 3, over = tiles & 7;
+    const int tile = xcd * each + min(xcd, over) + (id >> 3);
+    const int band = tile / (kBand * tiles_n), in = tile - band * kBand * tiles_n;
+    const int high = min(kBand, tiles_m - band * kBand);  // tiles of M in this band
+    n = in / high;
+    m = band * kBand + in - n * high;
+  }
+};
+
+template <int TM, int TN, int WM, int WN, int BK, int NST, bool PONG, int ACT>
+__global__ __launch_bounds__(64 * WM * WN) void linear_f16_tiles(LinearF16Args a, int tiles_m, int tiles_n) {
+  using S = TileShape<TM, TN, WM, WN, BK, NST>;
+  constexpr int MB = S::MB, NB = S::NB;
+  __shared__ __attribute__((aligned(1024))) char lds[S::BYTES];
+  _Float16* const ring = reinterpret_cast<_Float16*>(lds);
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const TilePlace place(tiles_m, tiles_n);
+  const int m0 = place.m * TM, n0 = place.n * TN;
+  const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
+
+  // Load i of a wavefront fills block i * WAVES + wave of a stage, rows of W (the first TN) or of x: the bytes
+  // from the tile's first row to this lane's row and chunk of K.
+  constexpr int WLOADS = TN / S::ROWS / S::WAVES;  // loads of W, before those of x
+  static_assert(TN % (S::ROWS * S::WAVES) == 0, "a load takes rows of one operand");
+  const char* const wbase = reinterpret_cast<const char*>(a.w + static_cast<size_t>(n0) * a.K);
+  const char* const xbase = reinterpret_cast<const char*>(a.x + static_cast<size_t>(m0) * a.K);
+  uint32_t off[S::LOADS];
+#pragma unroll
+  for (int i = 0; i < S::LOADS; ++i) {
+    const int row = (i * S::WAVES + wave) * S::ROWS + lane / S::CPR - (i < WLOADS ? 0 : TN);
+    const int chunk = (lane % S::CPR) ^ sw<BK>(row);
+    off[i] = static_cast<uint32_t>(min(row, (i < WLOADS ? a.N - n0 : a.M - m0) - 1)) *
+                 static_cast<uint32_t>(2 * a.K) + 16 * chunk;
+  }
+  const int steps = (a.K + BK - 1) / BK;
+  auto issue = [&](int step) {
+    _Float16* const to = ring + step % NST * S::STAGE + wave * 512;
+    const int left = 2 * (a.K - step * BK);  // bytes of a row from here
+    if (left >= 2 * BK) {
+#pragma unroll
+      for (int i = 0; i < S::LOADS; ++i)
+        dma16_at((i < WLOADS ? wbase : xbase) + 2 * step * BK, off[i], to + i * S::WAVES * 512);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::LOADS; ++i) {
+        // chunks past K: the first of the tile (any; left out below)
+        const int row = (i * S::WAVES + wave) * S::ROWS + lane / S::CPR;
+        const int chunk = (lane % S::CPR) ^ sw<BK>(row);
+        dma16_at(i < WLOADS ? wbase : xbase, 16 * chunk < left ? off[i] + 2 * step * BK : 0u,
+                 to + i * S::WAVES * 512);
+      }
+    }
+  };
+
+  floatx16 acc[MB][NB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[mb][nb][e] = 0.0f;
+
+  const int whole = a.K / BK;
+  if constexpr (PONG) {
+    // Two groups of wavefronts, one of each on a SIMD, half a turn apart: while one reads its operands from
+    // LDS the other has the matrix pipe. Between two barriers a group either reads (2 k-steps of 16) and
+    // starts the copies of the stage after, or multiplies. Group 1 runs one barrier behind, so when group 0
+    // starts on a stage, group 1 has just read the last of the stage before: the copies into that one may
+    // start, and both have waited for their copies into this one.
+    constexpr int TURNS = BK / 32;
+    const int group = wave / (S::WAVES / 2);
+    // this wavefront's copies into the stage after `step` have landed
+    auto next_ready = [&](int step) {
+      if (step + NST - 1 < steps) wait_vmcnt<(NST - 2) * S::LOADS>();
+      else wait_vmcnt<0>();
+    };
+    auto turn = [&](int step, int c, auto tail) {
+      constexpr bool TAIL = decltype(tail)::value;
+      const _Float16* const ws = ring + step % NST * S::STAGE + (wn + r) * BK;
+      const _Float16* const xs = ring + step % NST * S::STAGE + (TN + wm + r) * BK;
+      half8 wf[2][NB], xf[2][MB];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = 2 * c + i, at = 8 * ((2 * k + h) ^ sw<BK>(r));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) wf[i][nb] = *reinterpret_cast<const half8*>(ws + 32 * nb * BK + at);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) xf[i][mb] = *reinterpret_cast<const half8*>(xs + 32 * mb * BK + at);
+        if (TAIL && step * BK + 16 * k + 8 * h >= a.K) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) wf[i][nb] = half8{};
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) xf[i][mb] = half8{};
+        }
+      }
+      if (c == 0 && step > 0 && step + NST - 1 < steps) issue(step + NST - 1);
+      wait_lgkmcnt<0>();
+      if (c == TURNS - 1 && group == 1) next_ready(step);
+      __builtin_amdgcn_sched_barrier(0);
+      stage_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            acc[mb][nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[i][nb], xf[i][mb], acc[mb][nb], 0, 0, 0);
+      __builtin_amdgcn_s_setprio(0);
+      if (c == TURNS - 1 && group == 0) next_ready(step);
+      __builtin_amdgcn_sched_barrier(0);
+      stage_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < NST; ++i)
+      if (i < steps) issue(i);
+    if (steps >= NST) wait_vmcnt<(NST - 1) * S::LOADS>();
+    else wait_vmcnt<0>();
+    stage_barrier();
+    if (group == 1) stage_barrier();
+    for (int step = 0; step < whole; ++step) {
+#pragma unroll
+      for (int c = 0; c < TURNS; ++c) turn(step, c, std::false_type{});
+    }
+    if (whole < steps) {
+#pragma unroll
+      for (int c = 0; c < TURNS; ++c) turn(whole, c, std::true_type{});
+    }
+    if (group == 0) stage_barrier();
+  } else {
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+      if (i < steps) issue(i);
+    // One step; TAIL: the last one, with less than BK of K left.
+    auto take = [&](int step, auto tail) {
+      constexpr bool TAIL = decltype(tail)::value;
+      if (step + NST - 2 < steps) wait_vmcnt<(NST - 2) * S::LOADS>();
+      else wait_vmcnt<0>();
+      wait_lgkmcnt<0>();  // this wavefront's reads of the stage that is filled next
+      stage_barrier();
+      if (step + NST - 1 < steps) issue(step + NST - 1);
+      const _Float16* const ws = ring + step % NST * S::STAGE + (wn + r) * BK;
+      const _Float16* const xs = ring + step % NST * S::STAGE + (TN + wm + r) * BK;
+      half8 wf[2][NB], xf[2][MB];
+      auto read = [&](int s) {
+        const int at = 8 * ((2 * s + h) ^ sw<BK>(r));  // rows 32 apart share it
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) wf[s & 1][nb] = *reinterpret_cast<const half8*>(ws + 32 * nb * BK + at);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) xf[s & 1][mb] = *reinterpret_cast<const half8*>(xs + 32 * mb * BK + at);
+        if (TAIL && step * BK + 16 * s + 8 * h >= a.K) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) wf[s & 1][nb] = half8{};
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) xf[s & 1][mb] = half8{};
+        }
+      };
+      read(0);
+#pragma unroll
+      for (int s = 0; s < BK / 16; ++s) {
+        if (s + 1 < BK / 16) read(s + 1);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            acc[mb][nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[s & 1][nb], xf[s & 1][mb], acc[mb][nb], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+      }
+    };
+    for (int step = 0; step < whole; ++step) take(step, std::false_type{});
+    if (whole < steps) take(whole, std::true_type{});
+  }
+  wait_lgkmcnt<0>();
+  stage_barrier();  // the ring is read out: it takes the rows to be stored, 32 a wavefront at a time
+
+  // LDS serves a wavefront's accesses in order: its own rows need no barrier
+  float* const box = reinterpret_cast<float*>(lds) + wave * 32 * S::OUT;
+  constexpr int PER = TN / WN / 8;  // lanes of a row, eight columns each
+  const int c = lane % PER * 8, n = n0 + wn + c;
+  float bias[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<floatx4*>(box + r * S::OUT + 32 * nb + 8 * q + 4 * h) =
+            floatx4{acc[mb][nb][4 * q], acc[mb][nb][4 * q + 1], acc[mb][nb][4 * q + 2],
+                    acc[mb][nb][4 * q + 3]};
+#pragma unroll 1
+    for (int row = lane / PER; row < 32; row += 64 / PER) {
+      const floatx4 lo = *reinterpret_cast<const floatx4*>(box + row * S::OUT + c);
+      const floatx4 hi = *reinterpret_cast<const floatx4*>(box + row * S::OUT + c + 4);
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = activate<ACT>((j < 4 ? lo[j & 3] : hi[j & 3]) + bias[j]);
+      const int m = m0 + wm + 32 * mb + row;
+      if (m < a.M && n < a.N) store8(a, m, n, y);
+    }
+  }
+}
+
+// f(ACT) as a compile-time value
+template <typename F>
+void for_activation(int act, F&& f) {
+  switch (act) {
+    case kActRelu: return f(std::integral_constant<int, kActRelu>{});
+    case kActGelu: return f(std::integral_constant<int, kActGelu>{});
+    case kActGeluTanh: return f(std::integral_constant<int, kActGeluTanh>{});
+    case kActSilu: return f(std::integral_constant<int, kActSilu>{});
+    default: return f(std::integral_constant<int, kActNone>{});
+  }
+}
+
+template <int TM, int TN, int WM, int WN, int BK, int NST, bool PONG>
+hipError_t launch_tiles(const LinearF16Args& a, hipStream_t st) {
+  const int tm = (a.M + TM - 1) / TM, tn = (a.N + TN - 1) / TN;
+  for_activation(a.act, [&](auto act) {
+    linear_f16_tiles<TM, TN, WM, WN, BK, NST, PONG, decltype(act)::value>
+        <<<static_cast<unsigned>(tm) * static_cast<unsigned>(tn), 64 * WM * WN, 0, st>>>(a, tm, tn);
+  });
+  return hipGetLastError();
+}
+
+// Up to 32 rows of x: the weights are what is read, once, straight into registers. A workgroup
+// has 32 columns of out; its wavefronts take every WAVES-th 64 of K each, and their sums meet in LDS and
+// are added in that order. Needs K % 8 == 0.
+template <int WAVES, int ACT>
+__global__ __launch_bounds__(64 * WAVES) void linear_f16_rows(LinearF16Args a) {
+  constexpr int ROW = 36;  // floats of a staged row of 32 columns
+  __shared__ __attribute__((aligned(16))) float box[WAVES][32 * ROW];
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
+  const int n0 = blockIdx.x * 32;
+  const _Float16* const w = a.w + static_cast<size_t>(min(n0 + r, a.N - 1)) * a.K + 8 * h;
+  const _Float16* const x = a.x + static_cast<size_t>(min(r, a.M - 1)) * a.K + 8 * h;
+  floatx16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll 2
+  for (int k = 64 * wave; k < a.K; k += 64 * WAVES) {
+    half8 wf[4], xf[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const bool in = k + 16 * s + 8 * h < a.K;
+      wf[s] = xf[s] = half8{};
+      if (in) {
+        wf[s] = *reinterpret_cast<const half8*>(w + k + 16 * s);
+        xf[s] = *reinterpret_cast<const half8*>(x + k + 16 * s);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[s], xf[s], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<floatx4*>(&box[wave][r * ROW + 8 * q + 4 * h]) =
+        floatx4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * 32; i += 64 * WAVES) {
+    const int m = i >> 5, n = n0 + (i & 31);
+    if (m >= a.M || n >= a.N) continue;
+    float y = box[0][m * ROW + (i & 31)];
+#pragma unroll
+    for (int g = 1; g < WAVES; ++g) y += box[g][m * ROW + (i & 31)];
+    y = activate<ACT>(y + (a.bias ? a.bias[n] : 0.0f));
+    const size_t at = static_cast<size_t>(m) * a.N + n;
+    if (a.residual) y += static_cast<float>(a.residual[at]);
+    if (a.out_f32) static_cast<float*>(a.out)[at] = y;
+    else static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(y);
+  }
+}
+
+template <int WAVES>
+hipError_t launch_rows(const LinearF16Args& a, hipStream_t st) {
+  for_activation(a.act, [&](auto act) {
+    linear_f16_rows<WAVES, decltype(act)::value>
+        <<<static_cast<unsigned>((a.N + 31) / 32), 64 * WAVES, 0, st>>>(a);
+  });
+  return hipGetLastError();
 }
 
 }  // namespace
 
+// The kernels and how long they take, in us, by the tiles that one round of the chip holds and the K of a
+// round, measured over M 8 .. 16384, N and K 384 .. 4096 (the fit holds within a tenth from one round on):
+//   rows    32 x 32, M <= 32        24 x 4096 x 1024 5.9 against 6.8 on 64 x 64; 64 rows 9.0 against 6.8
+//   64      512 a round             3.7 + 6.2 K / 1024    2048 x 1024 x 1024 10.0 (128: 12.4, 256: 26.9)
+//   128     256 a round             4.3 + 9.4 K / 1024    4096 x 1024 x 4096 42.1 (64: 55.6, 256: 87.3)
+//   128 x 2 512 a round, 2 a CU     5.2 + 15.5 K / 1024   2048 x 4096 x 1024 22.9 (128: 26.2, 256: 31.6)
+//   256     256 a round             7.0 + 28.5 K / 1024   16384 x 4096 x 1024 139.9 (128 x 2: 156.5)
 hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>((a.N + 63) / 64), static_cast<unsigned>((a.M + 63) / 64));
-  linear_f16_any<<<grid, 256, 0, st>>>(a);
-  return hipGetLastError();
+  if (a.K % 8) {
+    const int tm = (a.M + 63) / 64, tn = (a.N + 63) / 64;
+    for_activation(a.act, [&](auto act) {
+      linear_f16_any<decltype(act)::value>
+          <<<static_cast<unsigned>(tm) * static_cast<unsigned>(tn), 256, 0, st>>>(a, tn);
+    });
+    return hipGetLastError();
+  }
+  if (a.M <= 32) return launch_rows<8>(a, st);
+  const float k = static_cast<float>(a.K) / 1024.0f;
+  auto rounds = [&](int tile, int64_t slots) {
+    const int64_t tiles = int64_t{(a.M + tile - 1) / tile} * ((a.N + tile - 1) / tile);
+    return static_cast<float>((tiles + slots - 1) / slots);
+  };
+  const float by64 = rounds(64, 512) * (3.7f + 6.2f * k), by128 = rounds(128, 256) * (4.3f + 9.4f * k),
+              by128x2 = rounds(128, 512) * (5.2f + 15.5f * k), by256 = rounds(256, 256) * (7.0f + 28.5f * k);
+  const float least = fminf(fminf(by64, by128), fminf(by128x2, by256));
+  if (by64 == least) return launch_tiles<64, 64, 2, 2, 128, 2, false>(a, st);
+  if (by128 == least) return launch_tiles<128, 128, 2, 4, 128, 2, false>(a, st);
+  if (by128x2 == least) return launch_tiles<128, 128, 2, 2, 64, 2, false>(a, st);
+  return launch_tiles<256, 256, 2, 4, 64, 2, true>(a, st);
 }
 
 }  // namespace tessery

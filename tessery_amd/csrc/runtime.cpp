@@ -518,7 +518,7 @@ bool linear_f16_args(const Params& p, uint64_t threads, uint32_t group, void* co
   const uint64_t M = p.rows, N = p.cols, K = p.k;
   const uint32_t f = p.u1;
   if (group != 256 || threads != M || !M || M > (1u << 22) || !N || N > 65536 || !K ||
-      K > 65536 || p.u0 >= tessery::kActCount || (f & ~kLinearFlags))
+      K > 65536 || M * N >= (uint64_t{1} << 36) || p.u0 >= tessery::kActCount || (f & ~kLinearFlags))
     return false;
   if (sz[0] < M * K * 2 || sz[1] < N * K * 2 || ((f & kLinearBias) && sz[2] < N * 4) ||
       ((f & kLinearResidual) && sz[3] < M * N * 2) || sz[4] < M * N * (f & kLinearF32 ? 4 : 2))
@@ -1103,8 +1103,6 @@ hipError_t launch(Runtime* rt, const Op& op, const Beside& beside) {
       tessery::LinearF16Args a;
       if (!linear_f16_args(p, op.threads, op.group, op.ptr.data(), op.size.data(), &a))
         return hipErrorInvalidValue;
-      a.scratch = rt->dense_scratch;
-      a.scratch_floats = kDenseScratchFloats;
       return tessery::launch_linear_f16(a, st);
     }
     default:

@@ -85,6 +85,14 @@ def test_long_sides(runtime, m, n, k):
     check(runtime, 5, m, n, k, bias=True)
 
 
+@pytest.mark.parametrize("m,n,k", [(2048, 2048, 72), (2000, 2041, 128), (2048, 4096, 64),
+                                   (2010, 4090, 200), (4096, 4096, 64), (4000, 4104, 200),
+                                   (4001, 4099, 72)])
+def test_many_outputs(runtime, m, n, k):
+    """Products that fill the chip with tiles of 128 and 256."""
+    check(runtime, 8, m, n, k, bias=True, residual=True, activation="relu")
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_rows_and_columns_that_are_not_finite(runtime, m):
     """A row of x or of W that holds a NaN or an infinity reaches its own outputs alone."""
