@@ -46,73 +46,26 @@ __device__ __forceinline__ float activate(float y) {
   return y;
 }
 
-// Four consecutive columns n .. n + 3 of row m.
-template <int ACT>
-__device__ __forceinline__ void finish4(const LinearF16Args& a, int m, int n, floatx4 y) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (n + j >= a.N) return;
-    float r = activate<ACT>(y[j] + (a.bias ? a.bias[n + j] : 0.0f));
-    const size_t at = static_cast<size_t>(m) * a.N + n + j;
-    if (a.residual) r += static_cast<float>(a.residual[at]);
-    if (a.out_f32)
-      static_cast<float*>(a.out)[at] = r;
-    else
-      static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(r);
-  }
-}
+// Rows of K values begin at any even address where K is odd: 16-byte accesses that promise no more. The
+// memory system takes them at any address; a copy straight into LDS (dma16_at) is given aligned ones.
+typedef half8 half8_any __attribute__((aligned(2)));
+typedef floatx4 floatx4_any __attribute__((aligned(4)));
 
-// 64 x 64 outputs a workgroup, 32 x 32 a wavefront (v_mfma_f32_32x32x16_f16: lane (r = l % 32,
-// g = l / 32) supplies A[r][8g..8g+7] and B[8g..8g+7][r] and holds D[8a + 4g + c][r] in element
-// 4a + c), 32 of K at a time through registers into LDS. A is W and B is x, so that a lane's four
-// elements are neighbours in a row of out. Any M, N and K.
-template <int ACT>
-__global__ __launch_bounds__(256) void linear_f16_any(LinearF16Args a, int tiles_n) {
-  constexpr int KT = 32, ROW = KT + 8;
-  __shared__ __attribute__((aligned(16))) _Float16 ws[64 * ROW], xs[64 * ROW];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n0 = static_cast<int>(blockIdx.x) % tiles_n * 64, m0 = static_cast<int>(blockIdx.x) / tiles_n * 64;
-  const int lr = tid >> 2, lc = (tid & 3) * 8;
-  auto fetch = [&](const _Float16* p, int row, int rows, int k) {
-    half8 v = {};
-    if (row < rows) {
-      const _Float16* at = p + static_cast<size_t>(row) * a.K + k;
+// The eight values at p, of which the row has `left` (zeros behind them).
+__device__ __forceinline__ half8 load8(const _Float16* p, int left) {
+  if (left >= 8) return *reinterpret_cast<const half8_any*>(p);
+  half8 v = {};
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (k + j < a.K) v[j] = at[j];
-    }
-    return v;
-  };
-  floatx16 acc;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
-  const int nw = (wave & 1) * 32, mw = (wave >> 1) * 32, r = lane & 31, g = lane >> 5;
-  for (int k = 0; k < a.K; k += KT) {
-    const half8 wv = fetch(a.w, n0 + lr, a.N, k + lc), xv = fetch(a.x, m0 + lr, a.M, k + lc);
-    __syncthreads();
-    *reinterpret_cast<half8*>(ws + lr * ROW + lc) = wv;
-    *reinterpret_cast<half8*>(xs + lr * ROW + lc) = xv;
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < KT / 16; ++s) {
-      const half8 af = *reinterpret_cast<const half8*>(ws + (nw + r) * ROW + 16 * s + 8 * g);
-      const half8 bf = *reinterpret_cast<const half8*>(xs + (mw + r) * ROW + 16 * s + 8 * g);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, bf, acc, 0, 0, 0);
-    }
-  }
-  const int m = m0 + mw + r;
-  if (m >= a.M) return;
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    finish4<ACT>(a, m, n0 + nw + 8 * q + 4 * g,
-            floatx4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]});
+  for (int j = 0; j < 7; ++j)
+    if (j < left) v[j] = p[j];
+  return v;
 }
 
 // TM x TN outputs a workgroup of WM x WN wavefronts, K taken BK at a time through a ring of NST stages in
 // LDS that global_load_lds_dwordx4 fills NST - 1 stages ahead. A row of a stage is BK halves; its 16-byte
 // chunks are XORed with sw(row), so the 16 rows of a read fall on 16 bank groups. Rows past M or N read the
 // last row and are not stored; the chunks of a last stage past K are left out as the operands are read.
-// Needs K % 8 == 0.
+// Where K is no multiple of 8 the stages pass through registers instead, one ahead (STAGED; NST = 2).
 template <int BK>
 __device__ __forceinline__ int sw(int row) {
   static_assert(BK == 64 || BK == 128, "rows of a half or a whole line of banks");
@@ -138,21 +91,21 @@ __device__ __forceinline__ void store8(const LinearF16Args& a, int m, int n, con
   float r[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) r[j] = y[j];
-  if (a.N % 8 == 0) {
+  if (n + 8 <= a.N) {
     if (a.residual) {
-      const half8 v = *reinterpret_cast<const half8*>(a.residual + at);
+      const half8 v = *reinterpret_cast<const half8_any*>(a.residual + at);
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[j] += static_cast<float>(v[j]);
     }
     if (a.out_f32) {
-      floatx4* const o = reinterpret_cast<floatx4*>(static_cast<float*>(a.out) + at);
+      floatx4_any* const o = reinterpret_cast<floatx4_any*>(static_cast<float*>(a.out) + at);
       o[0] = floatx4{r[0], r[1], r[2], r[3]};
       o[1] = floatx4{r[4], r[5], r[6], r[7]};
     } else {
       half8 v;
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = static_cast<_Float16>(r[j]);
-      *reinterpret_cast<half8*>(static_cast<_Float16*>(a.out) + at) = v;
+      *reinterpret_cast<half8_any*>(static_cast<_Float16*>(a.out) + at) = v;
     }
     return;
   }
@@ -164,6 +117,10 @@ __device__ __forceinline__ void store8(const LinearF16Args& a, int m, int n, con
     else static_cast<_Float16*>(a.out)[at + j] = static_cast<_Float16>(r[j]);
   }
 }
+
+// How a workgroup's stages are filled and read: by copies into LDS, the same with its wavefronts in two
+// groups that take turns, or through registers.
+enum class Feed { kCopies, kTurns, kStaged };
 
 // Workgroups go round the eight XCDs, each with an L2 of its own: an XCD takes a run of tiles, walked in
 // bands of kBand tiles of M, so that the tiles that run on it together share rows of x and of W.
@@ -181,7 +138,7 @@ struct TilePlace {
   }
 };
 
-template <int TM, int TN, int WM, int WN, int BK, int NST, bool PONG, int ACT>
+template <int TM, int TN, int WM, int WN, int BK, int NST, Feed FEED, int ACT>
 __global__ __launch_bounds__(64 * WM * WN) void linear_f16_tiles(LinearF16Args a, int tiles_m, int tiles_n) {
   using S = TileShape<TM, TN, WM, WN, BK, NST>;
   constexpr int MB = S::MB, NB = S::NB;
@@ -236,7 +193,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_f16_tiles(LinearF16Args a
       for (int e = 0; e < 16; ++e) acc[mb][nb][e] = 0.0f;
 
   const int whole = a.K / BK;
-  if constexpr (PONG) {
+  if constexpr (FEED == Feed::kTurns) {
     // Two groups of wavefronts, one of each on a SIMD, half a turn apart: while one reads its operands from
     // LDS the other has the matrix pipe. Between two barriers a group either reads (2 k-steps of 16) and
     // starts the copies of the stage after, or multiplies. Group 1 runs one barrier behind, so when group 0
@@ -305,17 +262,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_f16_tiles(LinearF16Args a
     }
     if (group == 0) stage_barrier();
   } else {
-#pragma unroll
-    for (int i = 0; i < NST - 1; ++i)
-      if (i < steps) issue(i);
-    // One step; TAIL: the last one, with less than BK of K left.
-    auto take = [&](int step, auto tail) {
+    // the products of one stage; TAIL: the last one, with less than BK of K left
+    auto multiply = [&](int step, auto tail) {
       constexpr bool TAIL = decltype(tail)::value;
-      if (step + NST - 2 < steps) wait_vmcnt<(NST - 2) * S::LOADS>();
-      else wait_vmcnt<0>();
-      wait_lgkmcnt<0>();  // this wavefront's reads of the stage that is filled next
-      stage_barrier();
-      if (step + NST - 1 < steps) issue(step + NST - 1);
       const _Float16* const ws = ring + step % NST * S::STAGE + (wn + r) * BK;
       const _Float16* const xs = ring + step % NST * S::STAGE + (TN + wm + r) * BK;
       half8 wf[2][NB], xf[2][MB];
@@ -345,8 +294,46 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_f16_tiles(LinearF16Args a
         __builtin_amdgcn_s_setprio(0);
       }
     };
-    for (int step = 0; step < whole; ++step) take(step, std::false_type{});
-    if (whole < steps) take(whole, std::true_type{});
+    if constexpr (FEED == Feed::kCopies) {
+      auto take = [&](int step, auto tail) {
+        if (step + NST - 2 < steps) wait_vmcnt<(NST - 2) * S::LOADS>();
+        else wait_vmcnt<0>();
+        wait_lgkmcnt<0>();  // this wavefront's reads of the stage that is filled next
+        stage_barrier();
+        if (step + NST - 1 < steps) issue(step + NST - 1);
+        multiply(step, tail);
+      };
+#pragma unroll
+      for (int i = 0; i < NST - 1; ++i)
+        if (i < steps) issue(i);
+      for (int step = 0; step < whole; ++step) take(step, std::false_type{});
+      if (whole < steps) take(whole, std::true_type{});
+    } else {
+      static_assert(NST == 2, "one stage ahead");
+      half8 held[S::LOADS];
+      auto fetch = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i) {
+          const int row = (i * S::WAVES + wave) * S::ROWS + lane / S::CPR;
+          const int at = step * BK + 8 * ((lane % S::CPR) ^ sw<BK>(row));
+          held[i] = load8(reinterpret_cast<const _Float16*>((i < WLOADS ? wbase : xbase) + off[i]) + step * BK,
+                          a.K - at);
+        }
+      };
+      auto store = [&](int step) {
+        _Float16* const to = ring + step % NST * S::STAGE + wave * 512 + lane * 8;
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i) *reinterpret_cast<half8*>(to + i * S::WAVES * 512) = held[i];
+      };
+      fetch(0);
+      store(0);
+      for (int step = 0; step < steps; ++step) {
+        __syncthreads();
+        if (step + 1 < steps) fetch(step + 1);
+        multiply(step, std::false_type{});  // what lies past K is zeros
+        if (step + 1 < steps) store(step + 1);
+      }
+    }
   }
   wait_lgkmcnt<0>();
   stage_barrier();  // the ring is read out: it takes the rows to be stored, 32 a wavefront at a time
@@ -392,11 +379,11 @@ void for_activation(int act, F&& f) {
   }
 }
 
-template <int TM, int TN, int WM, int WN, int BK, int NST, bool PONG>
+template <int TM, int TN, int WM, int WN, int BK, int NST, Feed FEED>
 hipError_t launch_tiles(const LinearF16Args& a, hipStream_t st) {
   const int tm = (a.M + TM - 1) / TM, tn = (a.N + TN - 1) / TN;
   for_activation(a.act, [&](auto act) {
-    linear_f16_tiles<TM, TN, WM, WN, BK, NST, PONG, decltype(act)::value>
+    linear_f16_tiles<TM, TN, WM, WN, BK, NST, FEED, decltype(act)::value>
         <<<static_cast<unsigned>(tm) * static_cast<unsigned>(tn), 64 * WM * WN, 0, st>>>(a, tm, tn);
   });
   return hipGetLastError();
@@ -404,7 +391,7 @@ hipError_t launch_tiles(const LinearF16Args& a, hipStream_t st) {
 
 // Up to 32 rows of x: the weights are what is read, once, straight into registers. A workgroup
 // has 32 columns of out; its wavefronts take every WAVES-th 64 of K each, and their sums meet in LDS and
-// are added in that order. Needs K % 8 == 0.
+// are added in that order.
 template <int WAVES, int ACT>
 __global__ __launch_bounds__(64 * WAVES) void linear_f16_rows(LinearF16Args a) {
   constexpr int ROW = 36;  // floats of a staged row of 32 columns
@@ -421,12 +408,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear_f16_rows(LinearF16Args a) {
     half8 wf[4], xf[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const bool in = k + 16 * s + 8 * h < a.K;
-      wf[s] = xf[s] = half8{};
-      if (in) {
-        wf[s] = *reinterpret_cast<const half8*>(w + k + 16 * s);
-        xf[s] = *reinterpret_cast<const half8*>(x + k + 16 * s);
-      }
+      const int left = a.K - (k + 16 * s + 8 * h);
+      wf[s] = load8(w + k + 16 * s, left);
+      xf[s] = load8(x + k + 16 * s, left);
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[s], xf[s], acc, 0, 0, 0);
@@ -469,14 +453,6 @@ hipError_t launch_rows(const LinearF16Args& a, hipStream_t st) {
 //   128 x 2 512 a round, 2 a CU     5.2 + 15.5 K / 1024   2048 x 4096 x 1024 22.9 (128: 26.2, 256: 31.6)
 //   256     256 a round             7.0 + 28.5 K / 1024   16384 x 4096 x 1024 139.9 (128 x 2: 156.5)
 hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st) {
-  if (a.K % 8) {
-    const int tm = (a.M + 63) / 64, tn = (a.N + 63) / 64;
-    for_activation(a.act, [&](auto act) {
-      linear_f16_any<decltype(act)::value>
-          <<<static_cast<unsigned>(tm) * static_cast<unsigned>(tn), 256, 0, st>>>(a, tn);
-    });
-    return hipGetLastError();
-  }
   if (a.M <= 32) return launch_rows<8>(a, st);
   const float k = static_cast<float>(a.K) / 1024.0f;
   auto rounds = [&](int tile, int64_t slots) {
@@ -485,11 +461,14 @@ hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st) {
   };
   const float by64 = rounds(64, 512) * (3.7f + 6.2f * k), by128 = rounds(128, 256) * (4.3f + 9.4f * k),
               by128x2 = rounds(128, 512) * (5.2f + 15.5f * k), by256 = rounds(256, 256) * (7.0f + 28.5f * k);
+  if (a.K % 8)
+    return by64 <= by128 ? launch_tiles<64, 64, 2, 2, 128, 2, Feed::kStaged>(a, st)
+                         : launch_tiles<128, 128, 2, 4, 64, 2, Feed::kStaged>(a, st);
   const float least = fminf(fminf(by64, by128), fminf(by128x2, by256));
-  if (by64 == least) return launch_tiles<64, 64, 2, 2, 128, 2, false>(a, st);
-  if (by128 == least) return launch_tiles<128, 128, 2, 4, 128, 2, false>(a, st);
-  if (by128x2 == least) return launch_tiles<128, 128, 2, 2, 64, 2, false>(a, st);
-  return launch_tiles<256, 256, 2, 4, 64, 2, true>(a, st);
+  if (by64 == least) return launch_tiles<64, 64, 2, 2, 128, 2, Feed::kCopies>(a, st);
+  if (by128 == least) return launch_tiles<128, 128, 2, 4, 128, 2, Feed::kCopies>(a, st);
+  if (by128x2 == least) return launch_tiles<128, 128, 2, 2, 64, 2, Feed::kCopies>(a, st);
+  return launch_tiles<256, 256, 2, 4, 64, 2, Feed::kTurns>(a, st);
 }
 
 }  // namespace tessery
