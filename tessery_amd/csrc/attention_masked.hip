@@ -8,10 +8,11 @@
 // the span's start. kv head = h / (H / KV).
 #include "common.h"
 #include "kernels.h"
+#include "lds_dma.h"
 
 #include <math.h>
-#include <stdlib.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace tessery {
@@ -116,15 +117,24 @@ __device__ __forceinline__ float other_half(float x, bool take_max) {
   return take_max ? fmaxf(a, b) : a + b;
 }
 
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off));
-  return x;
+// Least and most over the 32 lanes of each half (both halves hold the same queries), by lane exchanges
+// in quads, in mirrored halves of 8 and 16 lanes, and between rows of 16.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true);
 }
-__device__ __forceinline__ int wave_max_int(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x = max(x, __shfl_xor(x, off));
-  return x;
+template <bool MOST>
+__device__ __forceinline__ int of_two(int a, int b) {
+  return MOST ? max(a, b) : min(a, b);
+}
+template <bool MOST>
+__device__ __forceinline__ int half_wave(int x) {
+  x = of_two<MOST>(x, dpp<0xB1>(x));   // quad_perm [1, 0, 3, 2]
+  x = of_two<MOST>(x, dpp<0x4E>(x));   // quad_perm [2, 3, 0, 1]
+  x = of_two<MOST>(x, dpp<0x141>(x));  // row_half_mirror
+  x = of_two<MOST>(x, dpp<0x140>(x));  // row_mirror
+  const auto p = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(x), static_cast<unsigned>(x), false, false);
+  return __builtin_amdgcn_readfirstlane(of_two<MOST>(static_cast<int>(p[0]), static_cast<int>(p[1])));
 }
 
 // Keys that some row of a wavefront attends (lo, hi) and keys that all its rows attend (all_lo, all_hi).
@@ -135,10 +145,10 @@ struct WaveKeys {
 __device__ __forceinline__ WaveKeys wave_keys(KeyRange r, bool row) {
   const bool some = row && r.lo < r.hi;
   WaveKeys w;
-  w.lo = wave_min(some ? r.lo : 0x7fffffff);
-  w.hi = wave_max_int(some ? r.hi : 0);
-  w.all_lo = wave_max_int(!row ? 0 : some ? r.lo : 0x7fffffff);
-  w.all_hi = wave_min(!row ? 0x7fffffff : some ? r.hi : 0);
+  w.lo = half_wave<false>(some ? r.lo : 0x7fffffff);
+  w.hi = half_wave<true>(some ? r.hi : 0);
+  w.all_lo = half_wave<true>(!row ? 0 : some ? r.lo : 0x7fffffff);
+  w.all_hi = half_wave<false>(!row ? 0x7fffffff : some ? r.hi : 0);
   return w;
 }
 
@@ -154,26 +164,50 @@ struct ScoreArgs {
   float cap2;    // cap log2 e
 };
 
-// Scores of one 32-key block as v (log2 units), still to be masked: element e of lane (query, h) is the
-// key 8 (e / 4) + 4 h + e % 4 of the block. rel: the key of element 0 less the query's position.
-template <bool CAP, int BIAS>
-__device__ __forceinline__ void score_block(floatx16& v, const ScoreArgs& s, float slope2, float rel,
-                                            const float* biases) {
+// What is done to the products before the softmax: nothing (they are scaled as exponents are taken), the cap
+// alone, or a cap or none and then a bias, told apart as the kernel runs. (With the cap alone told apart there
+// too, 2 x 4096 with 16 heads of 128, a cap and a window took 143 us instead of 119.)
+enum class Scores { kPlain, kCapped, kAny };
+
+// Scores of one 32-key block, from products to log2 units, still to be masked: element e of lane (query, h)
+// is the key 8 (e / 4) + 4 h + e % 4 of the block. rel: the key of element 0 less the query's position.
+template <Scores HOW>
+__device__ __forceinline__ void score_block(floatx16& v, const MaskedArgs& a, const ScoreArgs& s,
+                                            float slope2, float rel, const float* biases) {
+  if (HOW == Scores::kCapped || a.cap > 0.0f) {
+    // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int c = 8 * (e >> 2) + (e & 3);
-    float x = v[e];
-    if constexpr (CAP) {
-      // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0
-      const float t = __builtin_amdgcn_exp2f(x * s.scale2);
-      x = fmaf(-2.0f * s.cap2, __builtin_amdgcn_rcpf(t + 1.0f), s.cap2);
-    } else if constexpr (BIAS != kBiasNone) {
-      x *= s.scale2;
+    for (int e = 0; e < 16; ++e) {
+      const float t = __builtin_amdgcn_exp2f(v[e] * s.scale2);
+      v[e] = fmaf(-2.0f * s.cap2, __builtin_amdgcn_rcpf(t + 1.0f), s.cap2);
     }
-    if constexpr (BIAS == kBiasSlopes) x = fmaf(-slope2, fabsf(rel + static_cast<float>(c)), x);
-    if constexpr (BIAS == kBiasTable) x += biases[c];
-    v[e] = x;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] *= s.scale2;
   }
+  if constexpr (HOW == Scores::kCapped) return;
+  if (a.bias_kind == kBiasSlopes) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      v[e] = fmaf(-slope2, fabsf(rel + static_cast<float>(8 * (e >> 2) + (e & 3))), v[e]);
+  }
+  if (a.bias_kind == kBiasTable) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] += biases[8 * (e >> 2) + (e & 3)];
+  }
+}
+
+// The batch row of a rank by falling length (equal ones in order); of up to 64 rows.
+__device__ __forceinline__ int row_of_rank(const MaskedArgs& a, int rank) {
+  if (a.B == 1 || a.B > 64) return rank;
+  const int lane = threadIdx.x & 63;
+  const uint32_t mine = lane < a.B ? min(a.lengths[lane], static_cast<uint32_t>(a.S)) : 0;
+  int before = 0;
+  for (int n = 0; n < a.B; ++n) {
+    const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), n));
+    before += other > mine || (other == mine && n < lane);
+  }
+  return __ffsll(__ballot(lane < a.B && before == rank)) - 1;
 }
 
 // Where a workgroup of four wavefronts works: 4 / KS wavefronts of 32 queries of one head each, in KS
@@ -187,34 +221,49 @@ struct Place {
   KeyRange mine;   // the keys of query i
   WaveKeys keys;
 
-  __device__ __forceinline__ Place(const MaskedArgs& a, int (*ends)[2]) {
+  __device__ __forceinline__ explicit Place(const MaskedArgs& a) {
     lane = threadIdx.x & 63;
     r = lane & 31;
     h = lane >> 5;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     qw = wave % QW;
     group = wave / QW;
-    const int blocks = (a.S + QB - 1) / QB;
+    // Long work first: batch rows by falling length, blocks of queries from the last (under a causal mask the
+    // longest, and outermost there). Within that, key heads change fastest, so that neighbours, which start
+    // on different compute units, are alike, and where they are a multiple of eight the query heads of one
+    // meet on one XCD.
+    const int blocks = (a.S + QB - 1) / QB, share = a.H / a.KV;
     int at = static_cast<int>(blockIdx.x);
-    const int qb = blocks - 1 - at % blocks;  // the last (causally longest) blocks of a head first
-    at /= blocks;
-    head = at % a.H;
-    b = at / a.H;
-    kvh = head / (a.H / a.KV);
+    kvh = at % a.KV;
+    at /= a.KV;
+    head = kvh * share + at % share;
+    at /= share;
+    int block, rank;
+    if (a.mask == kMaskBidirectional) {
+      block = at % blocks;
+      rank = at / blocks;
+    } else {
+      rank = at % a.B;
+      block = at / a.B;
+    }
+    const int qb = blocks - 1 - block;
+    b = row_of_rank(a, rank);
     i0 = qb * QB;
     i = i0 + qw * 32 + r;
     row = i < a.S;
-    mine = key_range(a, b, min(i, a.S - 1));
-    keys = wave_keys(mine, row);
-    if (lane == 0) {
-      ends[wave][0] = keys.lo;
-      ends[wave][1] = keys.hi;
-    }
-    L = static_cast<int>(min(a.lengths[b], static_cast<uint32_t>(a.S)));
     token = static_cast<size_t>(b) * a.S;
   }
 
-  // the tiles of `size` keys that the workgroup walks; none where nothing is attended
+  // The keys of this lane's query and of the wavefront. (Loads, like the lengths that the order of rows
+  // takes: after those of Q, whose way is as long.)
+  __device__ __forceinline__ void look(const MaskedArgs& a) {
+    mine = key_range(a, b, min(i, a.S - 1));
+    keys = wave_keys(mine, row);
+    L = static_cast<int>(min(a.lengths[b], static_cast<uint32_t>(a.S)));
+  }
+
+  // the tiles of `size` keys that the workgroup walks, from the wavefronts' `ends`; none where nothing is
+  // attended
   __device__ __forceinline__ void tiles(const int (*ends)[2], int size, int* first, int* last) const {
     __syncthreads();
     int lo = ends[0][0], hi = ends[0][1];
@@ -227,14 +276,13 @@ struct Place {
     *last = (hi + size - 1) / size;
   }
 
-  // whether no row of this wavefront attends a key of the block of 32 from j0, and whether some row does
-  // not attend them all
-  __device__ __forceinline__ bool skips(int j0) const { return j0 >= keys.hi || j0 + 32 <= keys.lo; }
-  __device__ __forceinline__ bool partial(int j0) const {
-    return j0 < keys.all_lo || j0 + 32 > keys.all_hi;
+  // whether no row of this wavefront attends a key of j0 .. j0 + n - 1, and whether some row does not attend
+  // them all
+  __device__ __forceinline__ bool skips(int j0, int n) const { return j0 >= keys.hi || j0 + n <= keys.lo; }
+  __device__ __forceinline__ bool partial(int j0, int n) const {
+    return j0 < keys.all_lo || j0 + n > keys.all_hi;
   }
   __device__ __forceinline__ void mask(floatx16& s, int j0) const {
-    if (!partial(j0)) return;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int j = j0 + 8 * (e >> 2) + 4 * h + (e & 3);
@@ -257,11 +305,14 @@ struct Softmax {
       for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
   }
 
-  // takes in the block's largest score, `factor` times that of s
-  __device__ __forceinline__ void raise(const floatx16& s, float factor, float lift) {
-    float most = s[0];
+  // takes in the blocks' largest score, `factor` times that of s
+  template <int N>
+  __device__ __forceinline__ void raise(const floatx16 (&s)[N], float factor, float lift) {
+    float most = s[0][0];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) most = fmaxf(most, s[e]);
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) most = fmaxf(most, s[n][e]);
     most = other_half(most, true) * factor;
     const bool grow = most > top + kSlack;
     if (__any(grow)) {
@@ -303,9 +354,10 @@ struct Softmax {
         sum = sum * c0 + from[(BOX - 1) * 64] * c1;
         top = both;
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
+        for (int dt = 0; dt < NDT; ++dt) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * c0 + from[(16 * dt + e) * 64] * c1;
+        }
       }
     }
     return true;
@@ -346,327 +398,295 @@ struct Softmax {
   }
 };
 
-// Tiles of fp16 operands on v_mfma_f32_32x32x16_f16: lane (r = l % 32, h = l / 32) supplies A[r][8h ..
-// 8h + 7] and B[8h .. 8h + 7][r] and holds D[8a + 4h + c][r] in element 4a + c.
-//   S^T = K Q^T for blocks of 32 keys x 32 queries: a query's scores lie in the two lanes r and r + 32.
-//   O^T = V^T P^T for 16 keys x 32 channels at a time: a lane's probabilities 8s .. 8s + 7 (keys 16s + 4h
-//   .. + 3 and 16s + 8 + 4h .. + 3) are the B operand as they lie; the A operand takes the same keys of V
-//   by two transposed reads.
-// Four wavefronts: 4 / KS of them take 32 queries each and the KS groups every KS-th block of keys; the
-// groups' sums meet in LDS at the end. K and V tiles of KT keys pass through registers into two LDS
-// buffers, the next tile's loads in flight during the products; keys past the length become zeros.
-// DP: the head size up to a power of two, zeros behind D.
-template <int DP>
-struct F16Tile {
-  static constexpr int KT = DP == 256 ? 32 : 64;
-  static constexpr int KROW = DP + 8;             // halves: 16 rows' chunks fall on 16 bank groups
-  static constexpr int K = KT * KROW, V = KT * DP;
-  static constexpr int CHUNKS = KT * DP / 8 / 256;  // 16-byte pieces a thread stages of K (and of V)
-  static constexpr int BIASES = 192;              // distances of one tile, KT + 128 - 1
-  static constexpr int BYTES = 2 * (K + V) * 2 + 2 * BIASES * 4;
+// The tiles of one kernel: KT keys of K and V pass through a ring of NST stages in LDS, which
+// global_load_lds_dwordx4 fills in blocks of 1 KiB, NST - 1 tiles ahead; one barrier a tile (two of a ring of
+// one: fp32 tiles so wide that LDS holds one, whose products take far longer than the copy). Rows lie as in
+// memory, DP channels long (the head size up to 32, 64, 96, 128 or 256), their 16-byte chunks permuted so that
+// what an instruction reads falls on different banks: place_k and place_v. Keys past the length repeat the
+// last one and are masked; chunks past the head size repeat its last one, against zeros of Q or into channels
+// that are not stored. (What of that is not finite is put right with the rows that are not: Softmax::store.)
+template <bool F16, int DP, int KS>
+struct Tile {
+  typedef typename std::conditional<F16, _Float16, float>::type T;
+  static constexpr int SIZE = F16 ? 2 : 4;
+  static constexpr int NB = F16 && (KS == 1 ? DP <= 96 : KS == 2 && DP <= 64) ? 2 : 1;  // blocks of 32 keys a group takes of a tile
+  static constexpr int KT = 32 * KS * NB;
+  static constexpr int CPR = DP * SIZE / 16;           // chunks of a row
+  static constexpr int BYTES = KT * DP * SIZE;         // of K, and of V
+  static constexpr int BLOCKS = BYTES / 1024;
+  static constexpr int LOADS = BLOCKS / 2;             // copies a wavefront makes for a tile
+  static constexpr int NST = BYTES > 32768 ? 1 : !F16 ? 2 : BYTES <= 4096 ? 4 : BYTES <= 8192 ? 3 : 2;
+  static constexpr int BIASES = KT + 128;              // distances of one tile, KT + QB - 1
+  static constexpr int RING = NST * 2 * BYTES;
+  static_assert(BLOCKS % 4 == 0, "a copy takes rows of one operand");
+
+  // chunk c of key row r lies at this chunk of its row
+  __device__ static __forceinline__ int place_k(int r, int c) {
+    if (CPR == 4) return c ^ ((r >> 1) & 3);
+    if (CPR == 8) return c ^ ((r >> 1) & 7);
+    if (CPR == 12) return c ^ ((r >> 2) & 3);
+    if (CPR == 24) return c ^ ((r >> 1) & 7);
+    return c ^ (r & 15);
+  }
+  // fp16: the 64-byte units of four rows that a transposed read takes; fp32: the 128-byte units of two rows
+  // four apart that a step takes
+  __device__ static __forceinline__ int place_v(int r, int c) {
+    if (F16) return DP == 64 ? c ^ (4 * ((r >> 1) & 1)) : DP >= 128 ? c ^ (4 * (r & 3)) : c;
+    return DP == 32 || DP == 96 ? c : c ^ (8 * ((r >> 2) & 1));
+  }
+  // fp32 rows of 32 or 96 channels: neighbours change places instead
+  __device__ static __forceinline__ int row_v(int r) {
+    return !F16 && (DP == 32 || DP == 96) ? r ^ ((r >> 2) & 1) : r;
+  }
 };
-// 64-byte units of a V row, so that the four rows of a transposed read fall on different banks
-template <int DP>
-__device__ __forceinline__ int v_unit(int row) {
-  return DP >= 128 ? (row & 3) : DP == 64 ? ((row >> 1) & 1) : 0;
-}
 
-template <int DP, int KS, bool CAP, int BIAS>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f16(MaskedArgs a, ScoreArgs sc) {
-  using T = F16Tile<DP>;
-  constexpr int KT = T::KT, QB = 128 / KS, NS = DP / 16, NDT = DP / 32;
-  constexpr int NB = KT / 32 / KS;  // key blocks of a tile that one wavefront takes
-  static_assert(NB >= 1, "a block of keys for every group");
-  __shared__ __attribute__((aligned(16))) char lds[T::BYTES];
+// fp16 on v_mfma_f32_32x32x16_f16: lane (r = l % 32, h = l / 32) supplies A[r][8h .. 8h + 7] and B[8h .. 8h + 7][r]
+// and holds D[8a + 4h + c][r] in element 4a + c.
+//   S^T = K Q^T for blocks of 32 keys x 32 queries: a query's scores lie in the two lanes r and r + 32.
+//   O^T = V^T P^T for 16 keys x 32 channels at a time: a lane's probabilities 8s .. 8s + 7 (keys 16s + 4h .. + 3
+//   and 16s + 8 + 4h .. + 3) are the B operand as they lie; the A operand takes the same keys of V by two
+//   transposed reads.
+// fp32 on v_mfma_f32_32x32x2_f32 (A[r][h], B[h][r], D as above), products and probabilities in fp32:
+//   S^T: step s takes channels s and s + DP / 2, so that a lane's values of Q are neighbours.
+//   O^T: the two keys of step e are those of the lanes' element e.
+template <bool F16, int DP, int KS, Scores HOW>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Scores::kAny || DP < 128 : DP == 64) ? 3 : 2) void attn_masked_tiles(MaskedArgs a, ScoreArgs sc) {
+  using T = Tile<F16, DP, KS>;
+  using E = typename T::T;
+  constexpr int KT = T::KT, QB = 128 / KS, NDT = DP / 32, NST = T::NST;
+  constexpr int JOIN = (KS - 1) * (4 / KS) * Softmax<NDT>::BOX * 256;
+  constexpr int BIAS_BYTES = HOW == Scores::kAny ? 2 * T::BIASES * 4 : 0;
+  constexpr int BYTES = T::RING + BIAS_BYTES > JOIN ? T::RING + BIAS_BYTES : JOIN;
+  __shared__ __attribute__((aligned(1024))) char lds[BYTES];
   __shared__ int ends[4][2];
-  _Float16* const kt0 = reinterpret_cast<_Float16*>(lds);
-  _Float16* const vt0 = kt0 + 2 * T::K;
-  float* const bt0 = reinterpret_cast<float*>(vt0 + 2 * T::V);
+  float* const bt0 = reinterpret_cast<float*>(lds + T::RING);
 
-  const Place<KS> w(a, ends);
-  const int tid = threadIdx.x, lane = w.lane, r = w.r, h = w.h, i = w.i;
-  const int b = w.b, head = w.head, kvh = w.kvh, L = w.L;
-  const size_t token = w.token;
-  const int ic = min(i, a.S - 1);
-  const _Float16* const q = static_cast<const _Float16*>(a.q) + (token + ic) * a.q_row + head * a.D;
-  const _Float16* const k = static_cast<const _Float16*>(a.k) + token * a.k_row + kvh * a.D;
-  const _Float16* const v = static_cast<const _Float16*>(a.v) + token * a.v_row + kvh * a.D;
-
-  half8 qf[NS];
+  Place<KS> w(a);
+  const int lane = w.lane, r = w.r, h = w.h;
+  // Q, in the order its operand takes it: half8 s is channels 16s + 8h .., floatx4 c channels DP / 2 h + 4c ..
+  typedef typename std::conditional<F16, half8, floatx4>::type Piece;
+  constexpr int PER = 16 / T::SIZE, NQ = F16 ? DP / 16 : DP / 8;
+  Piece qf[NQ];
+  {
+    const E* const q = static_cast<const E*>(a.q) + (w.token + min(w.i, a.S - 1)) * a.q_row + w.head * a.D;
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    qf[s] = half8{};
-    if (16 * s + 8 * h < a.D) {
-      qf[s] = *reinterpret_cast<const half8*>(q + 16 * s + 8 * h);
-      if (sc.q_sign != 1.0f) qf[s] *= static_cast<_Float16>(sc.q_sign);
+    for (int s = 0; s < NQ; ++s) {
+      const int ch = F16 ? 16 * s + 8 * h : h * (DP / 2) + 4 * s;
+      qf[s] = Piece{};
+      if (ch < a.D) qf[s] = *reinterpret_cast<const Piece*>(q + ch);
     }
   }
-  const float slope2 = BIAS == kBiasSlopes ? a.bias[head] * kLog2e : 0.0f;
-  const float* const table =
-      BIAS == kBiasTable ? a.bias + head * (2 * static_cast<size_t>(a.radius) + 1) : nullptr;
+  const bool tabled = HOW == Scores::kAny && a.bias_kind == kBiasTable;
+  const float slope2 = HOW == Scores::kAny && a.bias_kind == kBiasSlopes ? a.bias[w.head] * kLog2e : 0.0f;
+  const float* const table = a.bias + w.head * (2 * static_cast<size_t>(a.radius) + 1);  // if tabled
+  w.look(a);
+  if (lane == 0) {
+    ends[w.wave][0] = w.keys.lo;
+    ends[w.wave][1] = w.keys.hi;
+  }
   int first, last;
   w.tiles(ends, KT, &first, &last);
 
-  // staging: thread t takes 16-byte pieces t, t + 256, ... of the tile
-  half8 kreg[T::CHUNKS], vreg[T::CHUNKS];
-  float breg = 0.0f;
-  auto fetch = [&](int tile) {
+  // copy i of a wavefront fills block 4 i + wave of a stage: K, then V
+  const char* const kplane = reinterpret_cast<const char*>(static_cast<const E*>(a.k) + w.token * a.k_row + w.kvh * a.D);
+  const char* const vplane = reinterpret_cast<const char*>(static_cast<const E*>(a.v) + w.token * a.v_row + w.kvh * a.D);
+  const int krow = a.k_row * T::SIZE, vrow = a.v_row * T::SIZE, chunks = a.D * T::SIZE / 16;
+  auto issue = [&](int tile, int stage) {
+    const char* const kt = kplane + static_cast<size_t>(tile) * KT * krow;
+    const char* const vt = vplane + static_cast<size_t>(tile) * KT * vrow;
+    const int most = w.L - 1 - tile * KT;
+    int mine = lane;
+    // wide fp32 tiles: up to 32 offsets, made again for each tile rather than kept in registers
+    if constexpr (!F16 && DP >= 96) asm volatile("" : "+v"(mine));
 #pragma unroll
-    for (int c = 0; c < T::CHUNKS; ++c) {
-      const int piece = tid + 256 * c, key = tile * KT + piece / (DP / 8), ch = piece % (DP / 8) * 8;
-      kreg[c] = vreg[c] = half8{};
-      if (key < L && ch < a.D) {
-        kreg[c] = *reinterpret_cast<const half8*>(k + static_cast<size_t>(key) * a.k_row + ch);
-        vreg[c] = *reinterpret_cast<const half8*>(v + static_cast<size_t>(key) * a.v_row + ch);
-      }
-    }
-    if constexpr (BIAS == kBiasTable) {
-      // entry x: distance key - query of tile * KT - i0 + x - (QB - 1)
-      const int away = tile * KT - w.i0 + tid - (QB - 1);
-      if (tid < KT + QB - 1) breg = log2_bias(table[min(max(away, -a.radius), a.radius) + a.radius]);
+    for (int i = 0; i < T::LOADS; ++i) {
+      constexpr int HALF = T::LOADS / 2;
+      const int at = ((i < HALF ? i : i - HALF) * 4 + w.wave) * 64 + mine;
+      const int row = i < HALF ? at / T::CPR : T::row_v(at / T::CPR);
+      const int c = min(i < HALF ? T::place_k(row, at % T::CPR) : T::place_v(row, at % T::CPR), chunks - 1);
+      dma16_at(i < HALF ? kt : vt,
+               __umul24(static_cast<uint32_t>(min(row, most)), static_cast<uint32_t>(i < HALF ? krow : vrow)) +
+                   16u * static_cast<uint32_t>(c),
+               reinterpret_cast<_Float16*>(lds + stage * 2 * T::BYTES + (i * 4 + w.wave) * 1024));
     }
   };
-  auto stage = [&](int buffer) {
-    _Float16* const kt = kt0 + buffer * T::K;
-    _Float16* const vt = vt0 + buffer * T::V;
-#pragma unroll
-    for (int c = 0; c < T::CHUNKS; ++c) {
-      const int piece = tid + 256 * c, key = piece / (DP / 8), ch = piece % (DP / 8);
-      *reinterpret_cast<half8*>(kt + key * T::KROW + 8 * ch) = kreg[c];
-      *reinterpret_cast<half8*>(vt + key * DP + 8 * (ch ^ (4 * v_unit<DP>(key)))) = vreg[c];
+  float bias = 0.0f;
+  auto fetch_bias = [&](int tile) {
+    // entry x: distance key - query of tile * KT - i0 + x - (QB - 1)
+    if (tabled) {
+      const int x = static_cast<int>(threadIdx.x), away = tile * KT - w.i0 + x - (QB - 1);
+      if (x < KT + QB - 1) bias = log2_bias(table[min(max(away, -a.radius), a.radius) + a.radius]);
     }
-    if constexpr (BIAS == kBiasTable)
-      if (tid < KT + QB - 1) bt0[buffer * T::BIASES + tid] = breg;
+  };
+  auto store_bias = [&](int buffer) {
+    if (tabled && static_cast<int>(threadIdx.x) < KT + QB - 1)
+      bt0[buffer * T::BIASES + threadIdx.x] = bias;
   };
 
   Softmax<NDT> soft;
-  if (first < last) {
-    fetch(first);
-    stage(0);
+#pragma unroll
+  for (int s = 0; s < NQ; ++s) {
+    if (sc.q_sign != 1.0f) qf[s] *= static_cast<E>(sc.q_sign);
+    // Q has come before the first copy goes out: the compiler does not see the copies, and a wait for Q that
+    // it placed among them would wait for all
+    asm volatile("" : "+v"(qf[s]));
   }
-  __syncthreads();
+  if (first < last) {
+    fetch_bias(first);
+    store_bias(0);
+  }
+#pragma unroll
+  for (int n = 0; n < NST - 1; ++n)
+    if (first + n < last) issue(first + n, n);
+  int stage = 0;
   for (int tile = first; tile < last; ++tile) {
-    const int buffer = (tile - first) & 1;
-    if (tile + 1 < last) fetch(tile + 1);
-    const _Float16* const kt = kt0 + buffer * T::K;
-    const _Float16* const vt = vt0 + buffer * T::V;
+    if constexpr (NST == 1) {
+      wait_lgkmcnt<0>();
+      stage_barrier();
+      issue(tile, 0);
+      wait_vmcnt<0>();
+      stage_barrier();
+    } else {
+      if (tile + NST - 2 < last) wait_vmcnt<(NST - 2) * T::LOADS>();
+      else wait_vmcnt<0>();
+      wait_lgkmcnt<0>();  // this wavefront's reads of the stage that is filled next
+      stage_barrier();
+      if (tile + NST - 1 < last) issue(tile + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+    }
+    if (tile + 1 < last) fetch_bias(tile + 1);
+    const E* const kt = reinterpret_cast<const E*>(lds + stage * 2 * T::BYTES);
+    const E* const vt = reinterpret_cast<const E*>(lds + stage * 2 * T::BYTES + T::BYTES);
+    const int kb = w.group * T::NB * 32, j0 = tile * KT + kb;
+    if (!w.skips(j0, 32 * T::NB)) {  // wavefront-uniform
+      floatx16 s[T::NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int kb = (KS == 1 ? nb : w.group) * 32, j0 = tile * KT + kb;
-      if (w.skips(j0)) continue;  // wavefront-uniform
-      floatx16 s;
+      for (int nb = 0; nb < T::NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+        for (int e = 0; e < 16; ++e) s[nb][e] = 0.0f;
 #pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        const half8 kf = *reinterpret_cast<const half8*>(kt + (kb + r) * T::KROW + 16 * st + 8 * h);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], s, 0, 0, 0);
+      for (int nb = 0; nb < T::NB; ++nb)
+#pragma unroll
+        for (int st = 0; st < NQ; ++st) {
+          const int c = F16 ? 2 * st + h : h * (T::CPR / 2) + st;
+          const Piece kf = *reinterpret_cast<const Piece*>(kt + (kb + 32 * nb + r) * DP + PER * T::place_k(r, c));
+          if constexpr (F16) {
+            s[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], s[nb], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              s[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[st][j], s[nb], 0, 0, 0);
+          }
+        }
+#pragma unroll
+      for (int nb = 0; nb < T::NB; ++nb) product_done(s[nb]);
+      if constexpr (HOW != Scores::kPlain) {
+#pragma unroll
+        for (int nb = 0; nb < T::NB; ++nb)
+          score_block<HOW>(s[nb], a, sc, slope2, static_cast<float>(j0 + 32 * nb + 4 * h - w.i),
+                      bt0 + ((tile - first) & 1) * T::BIASES + kb + 32 * nb + 4 * h + QB - 1 - (w.qw * 32 + r));
       }
-      product_done(s);
-      score_block<CAP, BIAS>(s, sc, slope2, static_cast<float>(j0 + 4 * h - i),
-                             bt0 + buffer * T::BIASES + kb + 4 * h + QB - 1 - (w.qw * 32 + r));
-      w.mask(s, j0);
-      constexpr bool RAW = !CAP && BIAS == kBiasNone;  // still to be multiplied by scale2
-      soft.raise(s, RAW ? sc.scale2 : 1.0f, kLift);
-      half8 p[2];
+      if (w.partial(j0, 32 * T::NB)) {
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(RAW ? fmaf(s[e], sc.scale2, -soft.base) : s[e] - soft.base);
-        const float p1 =
-            __builtin_amdgcn_exp2f(RAW ? fmaf(s[e + 1], sc.scale2, -soft.base) : s[e + 1] - soft.base);
-        // fp16 probabilities for the product with V (they add 2^-12 of the output's own rounding,
-        // 2^-11, in the mean); the sum is that of the rounded ones, in fp32
-        const half2v two = __builtin_convertvector((float2v){p0, p1}, half2v);
-        p[e >> 3][e & 7] = two.x;
-        p[e >> 3][(e & 7) + 1] = two.y;
-        soft.sum = __builtin_amdgcn_fdot2(two, half2v{1, 1}, soft.sum, false);
+        for (int nb = 0; nb < T::NB; ++nb) w.mask(s[nb], j0 + 32 * nb);
       }
+      soft.raise(s, HOW == Scores::kPlain ? sc.scale2 : 1.0f, F16 ? kLift : 0.0f);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const int vrow = kb + 16 * st + 4 * h + ((lane & 15) >> 2);
-        const int ch = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      for (int nb = 0; nb < T::NB; ++nb) {
+        auto probability = [&](int e) {
+          return __builtin_amdgcn_exp2f(HOW == Scores::kPlain ? fmaf(s[nb][e], sc.scale2, -soft.base)
+                                                              : s[nb][e] - soft.base);
+        };
+        const int kn = kb + 32 * nb;
+        if constexpr (F16) {
+          half8 p[2];
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) {
-          const half4 v0 = read_transposed(vt + vrow * DP + 32 * (dt ^ v_unit<DP>(vrow)) + ch);
-          const half4 v1 =
-              read_transposed(vt + (vrow + 8) * DP + 32 * (dt ^ v_unit<DP>(vrow + 8)) + ch);
-          const half8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-          soft.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[st], soft.o[dt], 0, 0, 0);
+          for (int e = 0; e < 16; e += 2) {
+            // fp16 probabilities for the product with V: their rounding, averaged over the keys, is of the size
+            // of the output's own. The sum is that of the rounded ones, in fp32.
+            const half2v two = __builtin_convertvector((float2v){probability(e), probability(e + 1)}, half2v);
+            p[e >> 3][e & 7] = two.x;
+            p[e >> 3][(e & 7) + 1] = two.y;
+            soft.sum = __builtin_amdgcn_fdot2(two, half2v{1, 1}, soft.sum, false);
+          }
+          const int at = kn + 4 * h + ((lane & 15) >> 2);  // the row that this lane names
+          const int in = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+          for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+              // rows 8 apart share their placing; chunk 4 dt is the block's first
+              const int ch = 8 * T::place_v(at + 16 * st, 4 * dt) + in;
+              const half4 v0 = read_transposed(vt + (at + 16 * st) * DP + ch);
+              const half4 v1 = read_transposed(vt + (at + 16 * st + 8) * DP + ch);
+              const half8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+              soft.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[st], soft.o[dt], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[nb][e] = probability(e);
+            soft.sum += s[nb][e];
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int at = kn + 8 * (e >> 2) + 4 * h + (e & 3);
+            const E* const vr = vt + T::row_v(at) * DP;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+              soft.o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[4 * T::place_v(at, 8 * dt) + r], s[nb][e], soft.o[dt], 0, 0, 0);
+          }
         }
       }
     }
-    if (tile + 1 < last) stage(buffer ^ 1);
-    __syncthreads();
+    if (tile + 1 < last) store_bias((tile + 1 - first) & 1);
+    stage = stage + 1 == NST ? 0 : stage + 1;
   }
-  static_assert((KS - 1) * (4 / KS) * Softmax<NDT>::BOX * 256 <= T::BYTES, "sums fit the tiles' LDS");
-  if (soft.join(w, reinterpret_cast<float*>(lds))) soft.template store<_Float16>(a, w);
-}
-
-// Tiles of fp32 operands on v_mfma_f32_32x32x2_f32: lane (r, h) supplies A[r][h] and B[h][r], D as above.
-//   S^T = K Q^T: step s takes channels s and s + DP / 2, so that a lane's values of Q are neighbours.
-//   O^T = V^T P^T: the two keys of step e are those of the lanes' element e. A row of V lies in LDS with its
-//   32-channel blocks interleaved, so one read gives a lane its channel of every block.
-// Everything is fp32: products, sums, probabilities.
-template <int DP>
-struct F32Tile {
-  static constexpr int KT = DP >= 128 ? 32 : 64;
-  static constexpr int KROW = DP + 4;
-  static constexpr int K = KT * KROW, V = KT * DP;
-  static constexpr int CHUNKS = KT * DP / 4 / 256;
-  static constexpr int BIASES = 192;
-  static constexpr int BYTES = (2 * (K + V) + 2 * BIASES) * 4;
-};
-
-template <int DP, int KS, bool CAP, int BIAS>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_masked_f32(MaskedArgs a, ScoreArgs sc) {
-  using T = F32Tile<DP>;
-  constexpr int KT = T::KT, QB = 128 / KS, NDT = DP / 32, HALF = DP / 2;
-  constexpr int NB = KT / 32 / KS;  // key blocks of a tile that one wavefront takes
-  static_assert(NB >= 1, "a block of keys for every group");
-  __shared__ __attribute__((aligned(16))) char lds[T::BYTES];
-  __shared__ int ends[4][2];
-  float* const kt0 = reinterpret_cast<float*>(lds);
-  float* const vt0 = kt0 + 2 * T::K;
-  float* const bt0 = vt0 + 2 * T::V;
-
-  const Place<KS> w(a, ends);
-  const int tid = threadIdx.x, r = w.r, h = w.h;
-  const int ic = min(w.i, a.S - 1);
-  const float* const q = static_cast<const float*>(a.q) + (w.token + ic) * a.q_row + w.head * a.D;
-  const float* const k = static_cast<const float*>(a.k) + w.token * a.k_row + w.kvh * a.D;
-  const float* const v = static_cast<const float*>(a.v) + w.token * a.v_row + w.kvh * a.D;
-  floatx4 qf[HALF / 4];
-#pragma unroll
-  for (int c = 0; c < HALF / 4; ++c) {
-    const int ch = h * HALF + 4 * c;
-    qf[c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (ch < a.D) qf[c] = *reinterpret_cast<const floatx4*>(q + ch) * sc.q_sign;
-  }
-  const float slope2 = BIAS == kBiasSlopes ? a.bias[w.head] * kLog2e : 0.0f;
-  const float* const table =
-      BIAS == kBiasTable ? a.bias + w.head * (2 * static_cast<size_t>(a.radius) + 1) : nullptr;
-  int first, last;
-  w.tiles(ends, KT, &first, &last);
-
-  floatx4 kreg[T::CHUNKS], vreg[T::CHUNKS];
-  float breg = 0.0f;
-  auto fetch = [&](int tile) {
-#pragma unroll
-    for (int c = 0; c < T::CHUNKS; ++c) {
-      const int piece = tid + 256 * c, key = tile * KT + piece / (DP / 4), ch = piece % (DP / 4) * 4;
-      kreg[c] = vreg[c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (key < w.L && ch < a.D) {
-        kreg[c] = *reinterpret_cast<const floatx4*>(k + static_cast<size_t>(key) * a.k_row + ch);
-        vreg[c] = *reinterpret_cast<const floatx4*>(v + static_cast<size_t>(key) * a.v_row + ch);
-      }
-    }
-    if constexpr (BIAS == kBiasTable) {
-      const int away = tile * KT - w.i0 + tid - (QB - 1);
-      if (tid < KT + QB - 1) breg = log2_bias(table[min(max(away, -a.radius), a.radius) + a.radius]);
-    }
-  };
-  auto stage = [&](int buffer) {
-    float* const kt = kt0 + buffer * T::K;
-    float* const vt = vt0 + buffer * T::V;
-#pragma unroll
-    for (int c = 0; c < T::CHUNKS; ++c) {
-      const int piece = tid + 256 * c, key = piece / (DP / 4), ch = piece % (DP / 4) * 4;
-      *reinterpret_cast<floatx4*>(kt + key * T::KROW + ch) = kreg[c];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        vt[key * DP + ((ch + j) & 31) * NDT + ((ch + j) >> 5)] = vreg[c][j];
-    }
-    if constexpr (BIAS == kBiasTable)
-      if (tid < KT + QB - 1) bt0[buffer * T::BIASES + tid] = breg;
-  };
-
-  Softmax<NDT> soft;
-  if (first < last) {
-    fetch(first);
-    stage(0);
-  }
-  __syncthreads();
-  for (int tile = first; tile < last; ++tile) {
-    const int buffer = (tile - first) & 1;
-    if (tile + 1 < last) fetch(tile + 1);
-    const float* const kt = kt0 + buffer * T::K;
-    const float* const vt = vt0 + buffer * T::V;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int kb = (KS == 1 ? nb : w.group) * 32, j0 = tile * KT + kb;
-      if (w.skips(j0)) continue;  // wavefront-uniform
-      floatx16 s;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < HALF / 4; ++c) {
-        const floatx4 kf = *reinterpret_cast<const floatx4*>(kt + (kb + r) * T::KROW + h * HALF + 4 * c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[c][j], s, 0, 0, 0);
-      }
-      product_done(s);
-      score_block<CAP, BIAS>(s, sc, slope2, static_cast<float>(j0 + 4 * h - w.i),
-                             bt0 + buffer * T::BIASES + kb + 4 * h + QB - 1 - (w.qw * 32 + r));
-      w.mask(s, j0);
-      constexpr bool RAW = !CAP && BIAS == kBiasNone;
-      soft.raise(s, RAW ? sc.scale2 : 1.0f, 0.0f);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[e] = __builtin_amdgcn_exp2f(RAW ? fmaf(s[e], sc.scale2, -soft.base) : s[e] - soft.base);
-        soft.sum += s[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float* const vr = vt + (kb + 8 * (e >> 2) + 4 * h + (e & 3)) * DP + r * NDT;
-        float vf[NDT];
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) vf[dt] = vr[dt];
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-          soft.o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[dt], s[e], soft.o[dt], 0, 0, 0);
-      }
-    }
-    if (tile + 1 < last) stage(buffer ^ 1);
-    __syncthreads();
-  }
-  static_assert((KS - 1) * (4 / KS) * Softmax<NDT>::BOX * 256 <= T::BYTES, "sums fit the tiles' LDS");
-  if (soft.join(w, reinterpret_cast<float*>(lds))) soft.template store<float>(a, w);
-}
-
-// f(CAP, BIAS) as compile-time values
-template <typename F>
-void for_scores(const MaskedArgs& a, F&& f) {
-  using None = std::integral_constant<int, kBiasNone>;
-  using Slopes = std::integral_constant<int, kBiasSlopes>;
-  using Table = std::integral_constant<int, kBiasTable>;
-  auto with = [&](auto cap) {
-    if (a.bias_kind == kBiasNone) f(cap, None{});
-    else if (a.bias_kind == kBiasSlopes) f(cap, Slopes{});
-    else f(cap, Table{});
-  };
-  if (a.cap > 0.0f) with(std::true_type{});
-  else with(std::false_type{});
+  wait_lgkmcnt<0>();
+  __syncthreads();  // the ring is read out
+  if (soft.join(w, reinterpret_cast<float*>(lds))) soft.template store<E>(a, w);
 }
 
 template <bool F16, int DP, int KS>
 hipError_t launch_tiles(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
   constexpr int QB = 128 / KS;
   const dim3 grid(static_cast<unsigned>(static_cast<uint64_t>(a.B) * a.H * ((a.S + QB - 1) / QB)));
-  for_scores(a, [&](auto cap, auto bias) {
-    if constexpr (F16)
-      attn_masked_f16<DP, KS, decltype(cap)::value, decltype(bias)::value><<<grid, 256, 0, st>>>(a, s);
-    else
-      attn_masked_f32<DP, KS, decltype(cap)::value, decltype(bias)::value><<<grid, 256, 0, st>>>(a, s);
-  });
+  if constexpr (F16 || DP < 256 || KS == 1)
+    if (a.bias_kind != kBiasNone) {
+      attn_masked_tiles<F16, DP, KS, Scores::kAny><<<grid, 256, 0, st>>>(a, s);
+      return hipGetLastError();
+    }
+  if (a.cap > 0.0f)
+    attn_masked_tiles<F16, DP, KS, Scores::kCapped><<<grid, 256, 0, st>>>(a, s);
+  else
+    attn_masked_tiles<F16, DP, KS, Scores::kPlain><<<grid, 256, 0, st>>>(a, s);
   return hipGetLastError();
 }
 
+// How the keys of a block of queries are shared out: KS groups of wavefronts, 128 / KS queries a workgroup.
+// More groups shorten the walk over the keys and fill a chip that few workgroups would leave idle, and read
+// K and V oftener. W: workgroups at KS = 1; in us, KS = 1, 2 and 4 (up to 128 channels):
+//   one block of keys at most             17 x 5, 36 heads of 128, fp32            23.3  35.4  41.6
+//   W <= 72, from 128 keys on             fp16 1 x 5720, 1 head of 32, documents   56.7  32.9  23.8
+//                                         fp32 3 x 1210, 2 heads of 64, causal    107.4  64.1  41.5
+//   W <= 512                              fp16 1 x 4096, 16 heads of 128, causal  131   110      -
+//                                         fp32 8 x 1589, 4 heads of 32, causal     95.8  71.3  77.8
+//     beyond                              fp16 5 x 1971, 8 heads of 64, W 640      64.1  76.0  94.2
+//   twice that with spans, up to 64 channels or from 96 in fp32 (a block's documents may lie far apart)
+//                                         fp16 1 x 8192, 12 heads of 64           103    89     -
+//   W <= 256 where one workgroup's tiles fill a compute unit (fp32 from 96 channels, 256 channels)
+//                                         fp32 10 x 1518, 4 heads of 128          208   120     -
+//     beyond                              fp16 26 x 402, 4 heads of 256, W 416     49.1  59.4   -
 template <bool F16, int DP>
 hipError_t launch_split(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
-  static const int ks = getenv("TESSERY_KS") ? atoi(getenv("TESSERY_KS")) : 1;
-  if constexpr (DP <= (F16 ? 128 : 64))
-    if (ks == 2) return launch_tiles<F16, DP, 2>(a, s, st);
+  constexpr bool FILLS = DP == 256 || (!F16 && DP >= 96);
+  const int64_t w = int64_t{a.B} * a.H * ((a.S + 127) / 128);
+  const int64_t reach = a.window ? std::min<int64_t>(a.S, 2 * int64_t{a.window} + 128) : a.S;
+  if constexpr (DP <= 128)
+    if (w <= 72 && reach >= 128) return launch_tiles<F16, DP, 4>(a, s, st);
+  // (with a bias, two groups of fp32 of 256 channels would not fit their registers: launch_tiles has none)
+  const bool two = F16 || DP < 256 || a.bias_kind == kBiasNone;
+  if (two && reach > 32 && w <= (FILLS ? 256 : 512) * (a.spans && (FILLS || DP <= 64) ? 2 : 1))
+    return launch_tiles<F16, DP, 2>(a, s, st);
   return launch_tiles<F16, DP, 1>(a, s, st);
 }
 
@@ -674,6 +694,7 @@ template <bool F16>
 hipError_t launch_sized(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
   if (a.D <= 32) return launch_split<F16, 32>(a, s, st);
   if (a.D <= 64) return launch_split<F16, 64>(a, s, st);
+  if (a.D <= 96) return launch_split<F16, 96>(a, s, st);
   if (a.D <= 128) return launch_split<F16, 128>(a, s, st);
   return launch_split<F16, 256>(a, s, st);
 }

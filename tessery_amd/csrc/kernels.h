@@ -296,7 +296,11 @@ struct LinearF16Args {
   const _Float16* residual;
   void* out;
   int M, N, K, act, out_f32;
+  float* scratch;  // fp32 sums of a product whose K is shared out (null: it is not)
+  size_t scratch_floats;
 };
+// Whether launch_linear_f16 would use a scratch of so many floats.
+bool linear_f16_in_parts(int M, int N, int K, size_t scratch_floats);
 hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st);
 
 }  // namespace tessery

@@ -122,13 +122,22 @@ __device__ __forceinline__ void store8(const LinearF16Args& a, int m, int n, con
 // groups that take turns, or through registers.
 enum class Feed { kCopies, kTurns, kStaged };
 
+// A product whose K is shared out: part p takes the k_each of K from p k_each and leaves its fp32 sums in
+// sums + p M N, for linear_f16_sum. One part: all of K, no sums.
+struct Split {
+  int parts, k_each;
+  float* sums;
+};
+
 // Workgroups go round the eight XCDs, each with an L2 of its own: an XCD takes a run of tiles, walked in
 // bands of kBand tiles of M, so that the tiles that run on it together share rows of x and of W.
 constexpr int kBand = 8;
 struct TilePlace {
-  int m, n;
-  __device__ __forceinline__ TilePlace(int tiles_m, int tiles_n) {
-    const int tiles = tiles_m * tiles_n, id = static_cast<int>(blockIdx.x);
+  int m, n, part;
+  __device__ __forceinline__ TilePlace(int tiles_m, int tiles_n, const Split& split) {
+    const int tiles = tiles_m * tiles_n;
+    part = static_cast<int>(blockIdx.x) / tiles;
+    const int id = static_cast<int>(blockIdx.x) - part * tiles;
     const int xcd = id & 7, each = tiles >> 3, over = tiles & 7;
     const int tile = xcd * each + min(xcd, over) + (id >> 3);
     const int band = tile / (kBand * tiles_n), in = tile - band * kBand * tiles_n;
@@ -139,30 +148,39 @@ struct TilePlace {
 };
 
 template <int TM, int TN, int WM, int WN, int BK, int NST, Feed FEED, int ACT>
-__global__ __launch_bounds__(64 * WM * WN) void linear_f16_tiles(LinearF16Args a, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(64 * WM * WN) void linear_f16_tiles(LinearF16Args a, int tiles_m, int tiles_n,
+                                                                  Split split) {
   using S = TileShape<TM, TN, WM, WN, BK, NST>;
   constexpr int MB = S::MB, NB = S::NB;
   __shared__ __attribute__((aligned(1024))) char lds[S::BYTES];
   _Float16* const ring = reinterpret_cast<_Float16*>(lds);
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const TilePlace place(tiles_m, tiles_n);
+  const TilePlace place(tiles_m, tiles_n, split);
   const int m0 = place.m * TM, n0 = place.n * TN;
+  const int row_k = a.K, k0 = place.part * split.k_each;  // values of a row, the first of this part
+  if (split.parts > 1) {
+    a.K = min(a.K - k0, split.k_each);  // from here on the part's
+    a.bias = nullptr;
+    a.residual = nullptr;
+    a.out = split.sums + static_cast<size_t>(place.part) * a.M * a.N;
+    a.out_f32 = 1;
+  }
   const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
 
   // Load i of a wavefront fills block i * WAVES + wave of a stage, rows of W (the first TN) or of x: the bytes
   // from the tile's first row to this lane's row and chunk of K.
   constexpr int WLOADS = TN / S::ROWS / S::WAVES;  // loads of W, before those of x
   static_assert(TN % (S::ROWS * S::WAVES) == 0, "a load takes rows of one operand");
-  const char* const wbase = reinterpret_cast<const char*>(a.w + static_cast<size_t>(n0) * a.K);
-  const char* const xbase = reinterpret_cast<const char*>(a.x + static_cast<size_t>(m0) * a.K);
+  const char* const wbase = reinterpret_cast<const char*>(a.w + static_cast<size_t>(n0) * row_k + k0);
+  const char* const xbase = reinterpret_cast<const char*>(a.x + static_cast<size_t>(m0) * row_k + k0);
   uint32_t off[S::LOADS];
 #pragma unroll
   for (int i = 0; i < S::LOADS; ++i) {
     const int row = (i * S::WAVES + wave) * S::ROWS + lane / S::CPR - (i < WLOADS ? 0 : TN);
     const int chunk = (lane % S::CPR) ^ sw<BK>(row);
     off[i] = static_cast<uint32_t>(min(row, (i < WLOADS ? a.N - n0 : a.M - m0) - 1)) *
-                 static_cast<uint32_t>(2 * a.K) + 16 * chunk;
+                 static_cast<uint32_t>(2 * row_k) + 16 * chunk;
   }
   const int steps = (a.K + BK - 1) / BK;
   auto issue = [&](int step) {
@@ -379,12 +397,55 @@ void for_activation(int act, F&& f) {
   }
 }
 
+// out = act(sums of all parts + bias) + residual, eight outputs a thread, the parts in order.
+template <int ACT>
+__global__ __launch_bounds__(256) void linear_f16_sum(LinearF16Args a, Split split) {
+  const size_t n = static_cast<size_t>(a.M) * a.N, at = (blockIdx.x * size_t{256} + threadIdx.x) * 8;
+  if (at >= n) return;
+  float y[8] = {};
+  const bool whole = at + 8 <= n;
+  for (int p = 0; p < split.parts; ++p) {
+    const float* const from = split.sums + p * n + at;
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const floatx4 v = *reinterpret_cast<const floatx4_any*>(from + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[j + i] += v[i];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at + j < n) y[j] += from[j];
+    }
+  }
+  int c = static_cast<int>(at % a.N);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (a.bias) y[j] += a.bias[c];
+    y[j] = activate<ACT>(y[j]);
+    c = c + 1 == a.N ? 0 : c + 1;
+  }
+  a.N = static_cast<int>(n < 0x7fffffff ? n : 0x7fffffff);  // one row of all outputs
+  store8(a, 0, static_cast<int>(at), y);
+}
+
 template <int TM, int TN, int WM, int WN, int BK, int NST, Feed FEED>
-hipError_t launch_tiles(const LinearF16Args& a, hipStream_t st) {
+hipError_t launch_tiles(const LinearF16Args& a, hipStream_t st, Split split = {1, 0, nullptr}) {
   const int tm = (a.M + TM - 1) / TM, tn = (a.N + TN - 1) / TN;
+  const unsigned grid = static_cast<unsigned>(tm) * static_cast<unsigned>(tn) * static_cast<unsigned>(split.parts);
+  if (split.parts > 1) {
+    linear_f16_tiles<TM, TN, WM, WN, BK, NST, FEED, kActNone><<<grid, 64 * WM * WN, 0, st>>>(a, tm, tn, split);
+    const size_t pieces = (static_cast<size_t>(a.M) * a.N + 7) / 8;
+    for_activation(a.act, [&](auto act) {
+      linear_f16_sum<decltype(act)::value>
+          <<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, st>>>(a, split);
+    });
+    return hipGetLastError();
+  }
   for_activation(a.act, [&](auto act) {
     linear_f16_tiles<TM, TN, WM, WN, BK, NST, FEED, decltype(act)::value>
-        <<<static_cast<unsigned>(tm) * static_cast<unsigned>(tn), 64 * WM * WN, 0, st>>>(a, tm, tn);
+        <<<grid, 64 * WM * WN, 0, st>>>(a, tm, tn, split);
   });
   return hipGetLastError();
 }
@@ -443,32 +504,74 @@ hipError_t launch_rows(const LinearF16Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-}  // namespace
-
 // The kernels and how long they take, in us, by the tiles that one round of the chip holds and the K of a
 // round, measured over M 8 .. 16384, N and K 384 .. 4096 (the fit holds within a tenth from one round on):
 //   rows    32 x 32, M <= 32        24 x 4096 x 1024 5.9 against 6.8 on 64 x 64; 64 rows 9.0 against 6.8
 //   64      512 a round             3.7 + 6.2 K / 1024    2048 x 1024 x 1024 10.0 (128: 12.4, 256: 26.9)
+//     its K in parts                + 4.5, and 3 us a MB of sums   363 x 68 x 6479 20.3 between events (60.1)
 //   128     256 a round             4.3 + 9.4 K / 1024    4096 x 1024 x 4096 42.1 (64: 55.6, 256: 87.3)
 //   128 x 2 512 a round, 2 a CU     5.2 + 15.5 K / 1024   2048 x 4096 x 1024 22.9 (128: 26.2, 256: 31.6)
 //   256     256 a round             7.0 + 28.5 K / 1024   16384 x 4096 x 1024 139.9 (128 x 2: 156.5)
-hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st) {
-  if (a.M <= 32) return launch_rows<8>(a, st);
-  const float k = static_cast<float>(a.K) / 1024.0f;
-  auto rounds = [&](int tile, int64_t slots) {
-    const int64_t tiles = int64_t{(a.M + tile - 1) / tile} * ((a.N + tile - 1) / tile);
-    return static_cast<float>((tiles + slots - 1) / slots);
+// Where K is no multiple of 8: 64 and 128, through registers.
+enum class Kind { kRows, k64, k128, k128x2, k256 };
+struct Choice {
+  Kind kind;
+  int parts;
+};
+
+float rounds(int64_t m, int64_t n, int64_t tile, int64_t parts, int64_t slots) {
+  return static_cast<float>(((m + tile - 1) / tile * ((n + tile - 1) / tile) * parts + slots - 1) / slots);
+}
+
+Choice choose(int M, int N, int K, size_t scratch_floats) {
+  if (M <= 32) return {Kind::kRows, 1};
+  const float k = static_cast<float>(K) / 1024.0f;
+  Choice best = {Kind::k64, 1};
+  float least = rounds(M, N, 64, 1, 512) * (3.7f + 6.2f * k);
+  auto offer = [&](Kind kind, int parts, float us) {
+    if (us < least) {
+      least = us;
+      best = {kind, parts};
+    }
   };
-  const float by64 = rounds(64, 512) * (3.7f + 6.2f * k), by128 = rounds(128, 256) * (4.3f + 9.4f * k),
-              by128x2 = rounds(128, 512) * (5.2f + 15.5f * k), by256 = rounds(256, 256) * (7.0f + 28.5f * k);
-  if (a.K % 8)
-    return by64 <= by128 ? launch_tiles<64, 64, 2, 2, 128, 2, Feed::kStaged>(a, st)
-                         : launch_tiles<128, 128, 2, 4, 64, 2, Feed::kStaged>(a, st);
-  const float least = fminf(fminf(by64, by128), fminf(by128x2, by256));
-  if (by64 == least) return launch_tiles<64, 64, 2, 2, 128, 2, Feed::kCopies>(a, st);
-  if (by128 == least) return launch_tiles<128, 128, 2, 4, 128, 2, Feed::kCopies>(a, st);
-  if (by128x2 == least) return launch_tiles<128, 128, 2, 2, 64, 2, Feed::kCopies>(a, st);
-  return launch_tiles<256, 256, 2, 4, 64, 2, Feed::kTurns>(a, st);
+  offer(Kind::k128, 1, rounds(M, N, 128, 1, 256) * (4.3f + 9.4f * k));
+  if (K % 8 == 0) {
+    offer(Kind::k128x2, 1, rounds(M, N, 128, 1, 512) * (5.2f + 15.5f * k));
+    offer(Kind::k256, 1, rounds(M, N, 256, 1, 256) * (7.0f + 28.5f * k));
+  }
+  const size_t sums = static_cast<size_t>(M) * N;
+  for (int parts = 2; parts <= 32 && parts * sums <= scratch_floats && parts * 128 <= K; ++parts)
+    offer(Kind::k64, parts, rounds(M, N, 64, parts, 512) * (3.7f + 6.2f * k / parts) + 4.5f +
+                                3.0f * static_cast<float>(parts * sums) * 4e-6f);
+  return best;
+}
+
+}  // namespace
+
+bool linear_f16_in_parts(int M, int N, int K, size_t scratch_floats) {
+  return choose(M, N, K, scratch_floats).parts > 1;
+}
+
+hipError_t launch_linear_f16(const LinearF16Args& a, hipStream_t st) {
+  const Choice c = choose(a.M, a.N, a.K, a.scratch ? a.scratch_floats : 0);
+  const bool staged = a.K % 8 != 0;
+  Split split = {c.parts, 0, a.scratch};
+  split.k_each = ((a.K + c.parts - 1) / c.parts + 127) / 128 * 128;
+  split.parts = (a.K + split.k_each - 1) / split.k_each;
+  switch (c.kind) {
+    case Kind::kRows:
+      return launch_rows<8>(a, st);
+    case Kind::k64:
+      return staged ? launch_tiles<64, 64, 2, 2, 128, 2, Feed::kStaged>(a, st, split)
+                    : launch_tiles<64, 64, 2, 2, 128, 2, Feed::kCopies>(a, st, split);
+    case Kind::k128:
+      return staged ? launch_tiles<128, 128, 2, 4, 64, 2, Feed::kStaged>(a, st)
+                    : launch_tiles<128, 128, 2, 4, 128, 2, Feed::kCopies>(a, st);
+    case Kind::k128x2:
+      return launch_tiles<128, 128, 2, 2, 64, 2, Feed::kCopies>(a, st);
+    default:
+      return launch_tiles<256, 256, 2, 4, 64, 2, Feed::kTurns>(a, st);
+  }
 }
 
 }  // namespace tessery

@@ -946,6 +946,12 @@ bool prepare(Runtime* rt, const Op& op) {
   const size_t sums_bytes = kDenseScratchFloats * sizeof(float);
   if (op.route == R_ATTENTION_F16_NORM_ROPE || op.route == R_NORM_ROPE_F16 || op.route == R_ROPE)
     return ensure_rope(rt, p.seq, p.dim, p.theta);
+  if (op.route == R_LINEAR_F16) {
+    if (tessery::linear_f16_in_parts(static_cast<int>(p.rows), static_cast<int>(p.cols),
+                                     static_cast<int>(p.k), kDenseScratchFloats))
+      (void)have_scratch(&rt->dense_scratch, sums_bytes);
+    return true;
+  }
   tessery::DenseJob dense;
   if (dense_job(op, &dense)) {
     if (tessery::matmul_reads_planes(dense, kDensePlanesBytes))
@@ -1103,6 +1109,8 @@ hipError_t launch(Runtime* rt, const Op& op, const Beside& beside) {
       tessery::LinearF16Args a;
       if (!linear_f16_args(p, op.threads, op.group, op.ptr.data(), op.size.data(), &a))
         return hipErrorInvalidValue;
+      a.scratch = rt->dense_scratch;
+      a.scratch_floats = kDenseScratchFloats;
       return tessery::launch_linear_f16(a, st);
     }
     default:

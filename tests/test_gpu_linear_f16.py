@@ -85,6 +85,16 @@ def test_long_sides(runtime, m, n, k):
     check(runtime, 5, m, n, k, bias=True)
 
 
+@pytest.mark.parametrize("m,n,k", [(33, 65, 4096), (70, 96, 8000), (363, 68, 6479), (100, 130, 2561),
+                                   (64, 64, 65536), (200, 37, 1000)])
+@pytest.mark.parametrize("out_dtype", ["f16", "f32"])
+def test_long_sums_of_few_outputs(runtime, m, n, k, out_dtype):
+    """K shared out between workgroups, the parts added in order."""
+    for place in (False, True) if out_dtype == "f16" else (False,):
+        check(runtime, 9, m, n, k, bias=True, residual=True, activation="silu", out_dtype=out_dtype,
+              place=place)
+
+
 @pytest.mark.parametrize("m,n,k", [(2048, 2048, 72), (2000, 2041, 128), (2048, 4096, 64),
                                    (2010, 4090, 200), (4096, 4096, 64), (4000, 4104, 200),
                                    (4001, 4099, 72)])
