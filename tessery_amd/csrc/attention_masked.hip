@@ -174,18 +174,23 @@ enum class Scores { kPlain, kCapped, kAny };
 template <Scores HOW>
 __device__ __forceinline__ void score_block(floatx16& v, const MaskedArgs& a, const ScoreArgs& s,
                                             float slope2, float rel, const float* biases) {
-  if (HOW == Scores::kCapped || a.cap > 0.0f) {
-    // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0
+  // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0
+  auto turned = [&](float x) {
+    return -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * s.scale2) + 1.0f);
+  };
+  if constexpr (HOW == Scores::kCapped) {
+    // without the 1, which no softmax sees, and the factor 2 cap, which the exponents take
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float t = __builtin_amdgcn_exp2f(v[e] * s.scale2);
-      v[e] = fmaf(-2.0f * s.cap2, __builtin_amdgcn_rcpf(t + 1.0f), s.cap2);
-    }
+    for (int e = 0; e < 16; ++e) v[e] = turned(v[e]);
+    return;
+  }
+  if (a.cap > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = fmaf(2.0f * s.cap2, turned(v[e]), s.cap2);
   } else {
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] *= s.scale2;
   }
-  if constexpr (HOW == Scores::kCapped) return;
   if (a.bias_kind == kBiasSlopes) {
 #pragma unroll
     for (int e = 0; e < 16; ++e)
@@ -476,6 +481,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Score
       if (ch < a.D) qf[s] = *reinterpret_cast<const Piece*>(q + ch);
     }
   }
+  // what a score is multiplied by as its exponent is taken
+  const float factor = HOW == Scores::kPlain ? sc.scale2 : HOW == Scores::kCapped ? 2.0f * sc.cap2 : 1.0f;
   const bool tabled = HOW == Scores::kAny && a.bias_kind == kBiasTable;
   const float slope2 = HOW == Scores::kAny && a.bias_kind == kBiasSlopes ? a.bias[w.head] * kLog2e : 0.0f;
   const float* const table = a.bias + w.head * (2 * static_cast<size_t>(a.radius) + 1);  // if tabled
@@ -589,12 +596,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Score
 #pragma unroll
         for (int nb = 0; nb < T::NB; ++nb) w.mask(s[nb], j0 + 32 * nb);
       }
-      soft.raise(s, HOW == Scores::kPlain ? sc.scale2 : 1.0f, F16 ? kLift : 0.0f);
+      soft.raise(s, factor, F16 ? kLift : 0.0f);
 #pragma unroll
       for (int nb = 0; nb < T::NB; ++nb) {
         auto probability = [&](int e) {
-          return __builtin_amdgcn_exp2f(HOW == Scores::kPlain ? fmaf(s[nb][e], sc.scale2, -soft.base)
-                                                              : s[nb][e] - soft.base);
+          return __builtin_amdgcn_exp2f(HOW == Scores::kAny ? s[nb][e] - soft.base : fmaf(s[nb][e], factor, -soft.base));
         };
         const int kn = kb + 32 * nb;
         if constexpr (F16) {
