@@ -38,8 +38,10 @@ def key_ranges(batch: int, seq: int, lengths: NDArray, *, mask: str, window: int
 def attention_masked(q: NDArray, k: NDArray, v: NDArray, lengths: NDArray, *, mask: str,
                      window: int = 0, cap: float = 0.0, scale: float | None = None,
                      prefix: NDArray | None = None, spans: NDArray | None = None,
-                     slopes: NDArray | None = None, table: NDArray | None = None):
-    """q [B,S,H,D], k and v [B,S,KV,D] -> (out, bound), both [B,S,H,D]. The bound, for operands of
+                     slopes: NDArray | None = None, table: NDArray | None = None,
+                     tokens: NDArray | None = None):
+    """q [B,S,H,D], k and v [B,S,KV,D] -> (out, bound), both [B,S,H,D] (of `tokens` alone where they
+    are given, zeros elsewhere). The bound, for operands of
     q's type (fp16: probabilities rounded to fp16 for the product with v, as well as the output):
       scores   4 sqrt(D) u scale sum|q k| for the sum, 8 u |s| for its scaling to log2 units, 16 u cap
                for the tanh, 4 u |bias|; an error d of the scores changes out by at most
@@ -55,7 +57,7 @@ def attention_masked(q: NDArray, k: NDArray, v: NDArray, lengths: NDArray, *, ma
     out = np.zeros(q.shape)
     bound = np.zeros(q.shape)
     for b in range(batch):
-        for i in range(seq):
+        for i in range(seq) if tokens is None else tokens:
             if hi[b, i] <= lo[b, i]:
                 continue
             j = np.arange(lo[b, i], hi[b, i])

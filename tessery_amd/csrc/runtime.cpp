@@ -409,7 +409,8 @@ bool masked_args(const Params& p, uint64_t threads, uint32_t group, void* const*
     return false;
   if (p.u0 > tessery::kMaskPrefix || (f & ~kMaskedFlags) ||
       ((f & kMaskedSlopes) && (f & kMaskedTable)) || p.rows > kMaxSeq ||
-      !std::isfinite(p.scale) || !std::isfinite(p.theta) || p.theta < 0.0f)
+      !std::isfinite(p.scale) || !std::isfinite(p.theta) || p.theta < 0.0f ||
+      (p.theta > 0.0f && p.theta < 1e-30f))
     return false;
   tessery::MaskedArgs a{};
   const int e = f & kMaskedF16 ? 2 : 4, wide = static_cast<int>((H + 2 * KV) * D);

@@ -246,6 +246,8 @@ def attention_norm_rope_plan(*, tokens: int, seq: int, heads: int, kv_heads: int
 
 # Head dimensions of attention_masked: multiples of 8 up to this.
 MASKED_MAX_DIM = 256
+# The least cap of its scores: 2 * log2(e) / cap is a factor of the kernel's, in fp32.
+MASKED_MIN_CAP = 1e-30
 MASKS = {"causal": 0, "bidirectional": 1, "prefix": 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
@@ -277,7 +279,7 @@ def attention_masked_plan(*, tokens: int, seq: int, heads: int, kv_heads: int, d
         raise InferenceError()
     scale = dim**-0.5 if scale is None else float(scale)
     cap = float(cap)
-    if not math.isfinite(scale) or not 0.0 <= cap < 3.4e38:
+    if not math.isfinite(scale) or not (cap == 0.0 or MASKED_MIN_CAP <= cap < 3.4e38):
         raise InferenceError()
     flags = (_F16_FLAG[precision] | 2 * spans | 4 * slopes | 8 * table | 16 * (packed is True)
              | 32 * (packed is not False))

@@ -234,6 +234,35 @@ def test_large_scores(runtime, precision):
 
 
 @pytest.mark.parametrize("precision", ["f16", "f32"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+@pytest.mark.parametrize("biased", [False, True])
+def test_scales_that_are_not_positive(runtime, precision, scale, cap, biased):
+    q, k, v = operands(22, 1, 100, 2, 2, 64, precision)
+    slopes = np.array([0.1, 0.02], np.float32) if biased else None
+    check(runtime, q, k, v, [100], mask="causal", scale=scale, cap=cap, slopes=slopes)
+
+
+@pytest.mark.parametrize("precision", ["f16", "f32"])
+@pytest.mark.parametrize("b,s,h,kv,d", [(70, 40, 2, 1, 32), (3, 700, 12, 12, 64), (1, 1500, 2, 2, 128),
+                                        (2, 600, 3, 1, 256), (6, 130, 16, 8, 96), (1, 900, 1, 1, 32)])
+def test_many_and_few_workgroups(runtime, precision, b, s, h, kv, d):
+    """Batches on either side of every rule that shares the keys of a block out, and more rows than
+    are put in order of length."""
+    q, k, v = operands(23, b, s, h, kv, d, precision)
+    lengths = np.random.default_rng(23).integers(1, s + 1, size=b)
+    rows = np.unique(np.random.default_rng(24).integers(0, s, size=12))
+    for kw in (dict(mask="causal"), dict(mask="bidirectional", cap=9.0),
+               dict(mask="causal", slopes=np.full(h, 0.05, np.float32))):
+        got = run(runtime, q, k, v, lengths, **kw).astype(np.float64)
+        assert np.isfinite(got).all()
+        for n in {0, b // 2, b - 1}:  # a few tokens of a few batch rows
+            one = slice(n, n + 1)
+            want, bound = ref.attention_masked(q[one], k[one], v[one], lengths[one], tokens=rows, **kw)
+            assert np.all(np.abs(got[n, rows] - want[0, rows]) <= bound[0, rows])
+
+
+@pytest.mark.parametrize("precision", ["f16", "f32"])
 def test_all_at_once(runtime, precision):
     q, k, v = operands(19, 2, 260, 8, 4, 128, precision)
     table = np.random.default_rng(19).standard_normal((8, 65)).astype(np.float32)

@@ -115,6 +115,14 @@ def test_steps_match_the_oracle_and_ways_to_run_them_each_other(runtime):
         for n in got:
             np.testing.assert_array_equal(one[n], got[n], err_msg=n)
 
+        with runtime.profile_kernels() as profile:
+            with runtime.command():
+                for step in layer.steps():
+                    step()
+        assert [r["kernel"] for r in profile] == ["linear_f16", "copy", "rotary", "attention_masked"] + \
+            3 * ["linear_f16"]
+        assert all(r["gpu_seconds"] > 0 for r in profile)
+
         other = Layer(runtime, 2)  # eager work between the replays, on the same scratch
         builds = runtime.diagnostics()["graph_builds"]
         try:

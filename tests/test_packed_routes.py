@@ -63,7 +63,7 @@ def test_attention_launch():
     dict(dim=60), dict(dim=264), dict(dim=0), dict(dim=64.0), dict(mask="other"),
     dict(mask="prefix"), dict(prefix="p"), dict(precision="bf16"), dict(packed="k"),
     dict(window=-1), dict(window=2**32), dict(window=1.5), dict(radius=4), dict(table="t", radius=-1),
-    dict(table="t", radius=2**20 + 1), dict(slopes="s", table="t"), dict(cap=-1.0),
+    dict(table="t", radius=2**20 + 1), dict(slopes="s", table="t"), dict(cap=-1.0), dict(cap=1e-31),
     dict(cap=math.inf), dict(cap=math.nan), dict(scale=math.inf), dict(scale=math.nan)])
 def test_attention_refusals(changes):
     with pytest.raises(InferenceError):
