@@ -6,6 +6,9 @@
 //   channels from rot on keep y
 // cos and sin of pos * frequency[c] (times a factor that long contexts may ask for) come from a table
 // that rotary_table fills once in float64, so the angle of a far position is as exact as a near one's.
+// Every channel of q and k is read and written once, and its arithmetic is a few operations: the bound is
+// HBM. 16384 tokens of 24 fp16 heads of 128 channels with norms, 201 MB, take 47.7 us, 4.2 TB/s (a copy of
+// 1 GiB reaches 5.15); one query of 24 tokens takes 4 us, of which nearly all is the launch.
 #include "common.h"
 #include "kernels.h"
 
@@ -92,15 +95,16 @@ __device__ __forceinline__ float run_sum(float x) {
   return x;
 }
 
-// Lanes of 16-byte pieces: C = 16 / sizeof(T) channels a piece, two pieces a lane, D / 2C lanes a head (TP:
-// up to a power of two, at most a wavefront). Lane j of the rotated channels holds pairs C j .. C j + C - 1 -
+// Lanes of pieces: C channels a piece (16 bytes, or 2 channels where the sizes ask for it), two pieces a lane,
+// D / 2C lanes a head (TP: up to a power of two, at most a wavefront). Lane j of the rotated channels holds pairs C j .. C j + C - 1 -
 // the pieces at C j and rot / 2 + C j, or, interleaved, the two from 2 C j - so the turn stays in the lane
 // and only the norm's sum crosses lanes. Blocks (x: tokens, y: parts of HP heads, those of q before those
 // of k); a thread reads its table entries and weights once for HP heads of its token.
-// Needs D and rot to be multiples of 2C and rows of 16-byte pieces.
-template <typename T, int TP, int HP, bool INTERLEAVED, bool NORM>
+// Needs D and rot to be multiples of 2C: rows are then whole pieces too.
+template <typename T, int C, int TP, int HP, bool INTERLEAVED, bool NORM>
 __global__ __launch_bounds__(256) void rotary_pieces(RotaryArgs a, int q_parts) {
-  constexpr int C = 16 / static_cast<int>(sizeof(T));
+  constexpr int F = C < 4 ? C : 4;  // floats a read of the table
+  typedef float few __attribute__((ext_vector_type(F)));
   typedef T piece __attribute__((ext_vector_type(C)));
   const int j = threadIdx.x % TP;
   const uint32_t token = blockIdx.x * (256 / TP) + threadIdx.x / TP;
@@ -134,11 +138,11 @@ __global__ __launch_bounds__(256) void rotary_pieces(RotaryArgs a, int q_parts) 
   if (turns && known) {
     const float* const row = a.table + static_cast<size_t>(pos) * a.rot + C * j;
 #pragma unroll
-    for (int c = 0; c < C; c += 4) {
-      const floatx4 u = *reinterpret_cast<const floatx4*>(row + c);
-      const floatx4 v = *reinterpret_cast<const floatx4*>(row + (a.rot >> 1) + c);
+    for (int c = 0; c < C; c += F) {
+      const few u = *reinterpret_cast<const few*>(row + c);
+      const few v = *reinterpret_cast<const few*>(row + (a.rot >> 1) + c);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
+      for (int m = 0; m < F; ++m) {
         cs[c + m] = u[m];
         sn[c + m] = v[m];
       }
@@ -217,37 +221,45 @@ __global__ __launch_bounds__(256) void rotary_pieces(RotaryArgs a, int q_parts) 
   }
 }
 
-template <typename T, int TP, int HP>
+template <typename T, int C, int TP, int HP>
 hipError_t launch_pieces(const RotaryArgs& a, hipStream_t st) {
   const int q_parts = (a.H + HP - 1) / HP, parts = q_parts + (a.KV + HP - 1) / HP;
   const dim3 grid((a.tokens + 256 / TP - 1) / (256 / TP), static_cast<unsigned>(parts));
   if (a.interleaved) {
-    if (a.q_norm) rotary_pieces<T, TP, HP, true, true><<<grid, 256, 0, st>>>(a, q_parts);
-    else rotary_pieces<T, TP, HP, true, false><<<grid, 256, 0, st>>>(a, q_parts);
+    if (a.q_norm) rotary_pieces<T, C, TP, HP, true, true><<<grid, 256, 0, st>>>(a, q_parts);
+    else rotary_pieces<T, C, TP, HP, true, false><<<grid, 256, 0, st>>>(a, q_parts);
   } else {
-    if (a.q_norm) rotary_pieces<T, TP, HP, false, true><<<grid, 256, 0, st>>>(a, q_parts);
-    else rotary_pieces<T, TP, HP, false, false><<<grid, 256, 0, st>>>(a, q_parts);
+    if (a.q_norm) rotary_pieces<T, C, TP, HP, false, true><<<grid, 256, 0, st>>>(a, q_parts);
+    else rotary_pieces<T, C, TP, HP, false, false><<<grid, 256, 0, st>>>(a, q_parts);
   }
   return hipGetLastError();
 }
 
-template <typename T, int TP>
+template <typename T, int C, int TP>
 hipError_t launch_lanes(const RotaryArgs& a, hipStream_t st) {
   // Four heads a thread share its table entries and weights: 16384 tokens of 24 heads of 128 with norms take
-  // 49.8 us (a head 66, two 52.4, eight 52). Few rows take a head a thread, so that the chip has work.
+  // 49.8 us (a head 66, two 52.4, eight 52; stores past the caches then took it to 47.7). Few rows take a
+  // head a thread, so that the chip has work.
   const bool few = static_cast<uint64_t>(a.tokens) * (a.H + a.KV) * TP < (1u << 20);
-  return few ? launch_pieces<T, TP, 1>(a, st) : launch_pieces<T, TP, 4>(a, st);
+  return few ? launch_pieces<T, C, TP, 1>(a, st) : launch_pieces<T, C, TP, 4>(a, st);
 }
 
 template <typename T>
 hipError_t launch_typed(const RotaryArgs& a, hipStream_t st) {
-  constexpr int C2 = 32 / static_cast<int>(sizeof(T));  // channels a lane
-  const int lanes = a.D / C2;
-  if (a.D % C2 == 0 && a.rot % C2 == 0 && lanes <= 64) {
-    if (lanes <= 4) return launch_lanes<T, 4>(a, st);
-    if (lanes <= 8) return launch_lanes<T, 8>(a, st);
-    if (lanes <= 16) return launch_lanes<T, 16>(a, st);
-    return lanes <= 32 ? launch_lanes<T, 32>(a, st) : launch_lanes<T, 64>(a, st);
+  constexpr int C = 16 / static_cast<int>(sizeof(T));
+  const int lanes = a.D / (2 * C);
+  if (a.D % (2 * C) == 0 && a.rot % (2 * C) == 0 && lanes <= 64) {
+    if (lanes <= 4) return launch_lanes<T, C, 4>(a, st);
+    if (lanes <= 8) return launch_lanes<T, C, 8>(a, st);
+    if (lanes <= 16) return launch_lanes<T, C, 16>(a, st);
+    return lanes <= 32 ? launch_lanes<T, C, 32>(a, st) : launch_lanes<T, C, 64>(a, st);
+  }
+  // Sizes that 16-byte pieces do not divide: 32 x 714 tokens of 8 heads of 80 channels, 40 of them rotated,
+  // in fp16 take 16.1 us in pieces of two channels (52.6 as a wavefront per row).
+  if (a.D % 4 == 0 && a.rot % 4 == 0 && a.D <= 256) {
+    if (a.D <= 32) return launch_lanes<T, 2, 8>(a, st);
+    if (a.D <= 64) return launch_lanes<T, 2, 16>(a, st);
+    return a.D <= 128 ? launch_lanes<T, 2, 32>(a, st) : launch_lanes<T, 2, 64>(a, st);
   }
   const uint64_t rows = static_cast<uint64_t>(a.tokens) * (a.H + a.KV);
   rotary_any<T><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(a);

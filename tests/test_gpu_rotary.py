@@ -113,6 +113,25 @@ def test_tokens(runtime, precision, batch, seq):
 
 
 @pytest.mark.parametrize("precision", ["f16", "f32"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rot", [(4, 4), (24, 8), (36, 20), (40, 20), (80, 20), (132, 4), (252, 124)])
+def test_pieces_of_two_channels(runtime, precision, layout, dim, rot):
+    for norm, place in ((False, False), (True, True)):
+        check(runtime, dim, 2, 19, 3, 2, dim, rot, precision, layout=layout, norm=norm, packed=True,
+              place=place)
+
+
+@pytest.mark.parametrize("precision", ["f16", "f32"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rot", [(20, 20), (36, 4), (40, 8), (80, 80)])
+def test_many_rows(runtime, precision, layout, dim, rot):
+    """So many that a thread takes several heads, of which the last part of q and of k is not full."""
+    for norm in (False, True):
+        check(runtime, rot, 3, 1801, 26, 3, dim, rot, precision, layout=layout, norm=norm, packed=True,
+              place=True)
+
+
+@pytest.mark.parametrize("precision", ["f16", "f32"])
 def test_positions_of_documents(runtime, precision):
     at = batching.document_positions([[30, 50, 5], [90]], 90)
     for kv in (2, 0):
