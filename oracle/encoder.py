@@ -43,8 +43,8 @@ def attention_masked(q: NDArray, k: NDArray, v: NDArray, lengths: NDArray, *, ma
     """q [B,S,H,D], k and v [B,S,KV,D] -> (out, bound), both [B,S,H,D] (of `tokens` alone where they
     are given, zeros elsewhere). The bound, for operands of
     q's type (fp16: probabilities rounded to fp16 for the product with v, as well as the output):
-      scores   4 sqrt(D) u scale sum|q k| for the sum, 8 u |s| for its scaling to log2 units, 16 u cap
-               for the tanh, 4 u |bias|; an error d of the scores changes out by at most
+      scores   4 sqrt(D) u scale sum|q k| for the sum, 8 u |s| for its scaling to log2 units, 16 u |s|
+               for the tanh (s capped; fp16 up to a cap of 256: 16 u cap), 4 u |bias|; an error d of the scores changes out by at most
                2 d sum p|v|
       exp, sums over n keys   (8 + 4 sqrt(n)) u sum p|v|, numerator and denominator
       fp16     u16 (sum p|v| + |out|) for the probabilities, u16 |out| for the output
@@ -68,7 +68,7 @@ def attention_masked(q: NDArray, k: NDArray, v: NDArray, lengths: NDArray, *, ma
             d = 4 * math.sqrt(dim) * U32 * abs(scale) * np.abs(prod).sum(-1) + 8 * U32 * np.abs(s)
             if cap:
                 s = cap * np.tanh(s / cap)
-                d = d + 16 * U32 * cap
+                d = d + 16 * U32 * (cap if half and cap <= 256 else np.abs(s))
             bias = np.zeros_like(s)
             if slopes is not None:
                 bias = -slopes.astype(np.float64)[None] * np.abs(j - i)[:, None]

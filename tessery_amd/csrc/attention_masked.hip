@@ -162,31 +162,57 @@ struct ScoreArgs {
   float q_sign;  // -1 for a negative scale, 0 for none
   float scale2;  // |scale| log2 e; with a cap the factor in front of tanh's exponent, 2 |scale| log2 e / cap
   float cap2;    // cap log2 e
+  bool coarse;   // the cap's tanh may be off by 2^-23 of the cap rather than of the score
 };
+
+// tanh of half of x ln 2, to about 4 units of 2^-24 relative: t / (t + 2) of t = 2^x - 1 = 2^n (2^f - 1) + 2^n - 1 with
+// n the integer next to x, where 2^f - 1 is a polynomial (minimax of the relative error on [-1/2, 1/2], 2^-25).
+// Keeps NaN.
+__device__ __forceinline__ float tanh_of_log2(float x) {
+  x = x > 64.0f ? 64.0f : x;
+  x = x < -64.0f ? -64.0f : x;
+  const float n = rintf(x), f = x - n;
+  float p = 0x1.39f2eap-13f;
+  p = fmaf(p, f, 0x1.5e8ac4p-10f);
+  p = fmaf(p, f, 0x1.3b34a0p-7f);
+  p = fmaf(p, f, 0x1.c6b084p-5f);
+  p = fmaf(p, f, 0x1.ebfbe0p-3f);
+  p = fmaf(p, f, 0x1.62e430p-1f) * f;
+  const float two = __builtin_amdgcn_ldexpf(1.0f, static_cast<int>(n));
+  const float t = fmaf(two, p, two - 1.0f);
+  return t * __builtin_amdgcn_rcpf(t + 2.0f);
+}
 
 // What is done to the products before the softmax: nothing (they are scaled as exponents are taken), the cap
 // alone, or a cap or none and then a bias, told apart as the kernel runs. (With the cap alone told apart there
 // too, 2 x 4096 with 16 heads of 128, a cap and a window took 143 us instead of 119.)
+// fp16 takes kCapped where the tanh may be coarse.
 enum class Scores { kPlain, kCapped, kAny };
 
 // Scores of one 32-key block, from products to log2 units, still to be masked: element e of lane (query, h)
 // is the key 8 (e / 4) + 4 h + e % 4 of the block. rel: the key of element 0 less the query's position.
-template <Scores HOW>
+template <bool F16, Scores HOW>
 __device__ __forceinline__ void score_block(floatx16& v, const MaskedArgs& a, const ScoreArgs& s,
                                             float slope2, float rel, const float* biases) {
-  // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0
+  // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0. Under fp16 probabilities
+  // (2^-11) that is nothing for the caps that coarse stands for; fp32 takes the tanh that is exact there too.
   auto turned = [&](float x) {
     return -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * s.scale2) + 1.0f);
   };
   if constexpr (HOW == Scores::kCapped) {
-    // without the 1, which no softmax sees, and the factor 2 cap, which the exponents take
+    // without the 1, which no softmax sees, and the factor 2 cap (fp32: cap), which the exponents take
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = turned(v[e]);
+    for (int e = 0; e < 16; ++e) v[e] = F16 ? turned(v[e]) : tanh_of_log2(v[e] * s.scale2);
     return;
   }
   if (a.cap > 0.0f) {
+    if (F16 && s.coarse) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = fmaf(2.0f * s.cap2, turned(v[e]), s.cap2);
+      for (int e = 0; e < 16; ++e) v[e] = fmaf(2.0f * s.cap2, turned(v[e]), s.cap2);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = s.cap2 * tanh_of_log2(v[e] * s.scale2);
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] *= s.scale2;
@@ -482,7 +508,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Score
     }
   }
   // what a score is multiplied by as its exponent is taken
-  const float factor = HOW == Scores::kPlain ? sc.scale2 : HOW == Scores::kCapped ? 2.0f * sc.cap2 : 1.0f;
+  const float factor = HOW == Scores::kPlain ? sc.scale2 : HOW == Scores::kCapped ? (F16 ? 2.0f : 1.0f) * sc.cap2 : 1.0f;
   const bool tabled = HOW == Scores::kAny && a.bias_kind == kBiasTable;
   const float slope2 = HOW == Scores::kAny && a.bias_kind == kBiasSlopes ? a.bias[w.head] * kLog2e : 0.0f;
   const float* const table = a.bias + w.head * (2 * static_cast<size_t>(a.radius) + 1);  // if tabled
@@ -593,7 +619,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Score
       if constexpr (HOW != Scores::kPlain) {
 #pragma unroll
         for (int nb = 0; nb < T::NB; ++nb)
-          score_block<HOW>(s[nb], a, sc, slope2, static_cast<float>(j0 + 32 * nb + 4 * h - w.i),
+          score_block<F16, HOW>(s[nb], a, sc, slope2, static_cast<float>(j0 + 32 * nb + 4 * h - w.i),
                       bt0 + ((tile - first) & 1) * T::BIASES + kb + 32 * nb + 4 * h + QB - 1 - (w.qw * 32 + r));
       }
       if (w.partial(j0, 32 * T::NB)) {
@@ -661,7 +687,7 @@ hipError_t launch_tiles(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st)
   constexpr int QB = 128 / KS;
   const dim3 grid(static_cast<unsigned>(static_cast<uint64_t>(a.B) * a.H * ((a.S + QB - 1) / QB)));
   if constexpr (F16 || DP < 256 || KS == 1)
-    if (a.bias_kind != kBiasNone) {
+    if (a.bias_kind != kBiasNone || (F16 && a.cap > 0.0f && !s.coarse)) {
       attn_masked_tiles<F16, DP, KS, Scores::kAny><<<grid, 256, 0, st>>>(a, s);
       return hipGetLastError();
     }
@@ -722,6 +748,8 @@ hipError_t launch_attention_masked(const MaskedArgs& a, hipStream_t st) {
   s.q_sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
   s.scale2 = a.cap > 0.0f ? 2.0f * size / a.cap : a.scale == 0.0f ? 1.0f : size;
   s.cap2 = a.cap * kLog2e;
+  // a score is then off by at most 256 x 2^-22 = 2^-14, its probability by an eighth of its rounding to fp16
+  s.coarse = a.f16 && a.cap <= 256.0f;
   return a.f16 ? launch_sized<true>(a, s, st) : launch_sized<false>(a, s, st);
 }
 

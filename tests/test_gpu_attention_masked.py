@@ -139,6 +139,17 @@ def test_caps(runtime, precision, cap, std):
 
 
 @pytest.mark.parametrize("precision", ["f16", "f32"])
+@pytest.mark.parametrize("cap", [256.0, 300.0, 1e5])
+@pytest.mark.parametrize("biased", [False, True])
+def test_wide_caps(runtime, precision, cap, biased):
+    """Caps far above the scores leave them as exact as they were (the fp32 bound holds that of every
+    cap: it goes with the score, not with the cap)."""
+    q, k, v = operands(30, 2, 100, 4, 2, 64, precision)
+    slopes = np.array([0.1, 0.02, 0.3, 0.0], np.float32) if biased else None
+    check(runtime, q, k, v, [100, 64], mask="bidirectional", cap=cap, slopes=slopes)
+
+
+@pytest.mark.parametrize("precision", ["f16", "f32"])
 @pytest.mark.parametrize("mask", ["causal", "bidirectional"])
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 def test_slopes(runtime, precision, mask, cap):
