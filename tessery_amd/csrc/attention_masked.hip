@@ -6,6 +6,14 @@
 // Every mask here is a range of keys: hi_i is the row's length, i + 1 (causal) or max(i + 1, prefix_b),
 // i + window and the end of the token's span, whichever is least; lo_i the most of 0, i - window + 1 and
 // the span's start. kv head = h / (H / KV).
+//
+// A workgroup of four wavefronts keeps the queries and their outputs in registers and walks tiles of keys that LDS
+// copies bring (Tile), with one pass of a softmax in fp32 (Softmax). Two products of 2 D operations a pair go to
+// MFMA, one exponential a pair (with a cap three transcendentals, at a quarter of the rate) to the vector units,
+// which bound it beside them: uniform rows of 8192, 16 fp16 heads of 128, run at about 800 TFLOP/s, of 2048, 48
+// heads of 64, at 670, in fp32 32 heads of 64 at 104 (a product of 8192^3 reaches 1355 and 153). 2 x 4096 with a cap
+// and a window of 1024 takes 116 us, of which the cap's two transcendentals are about a third; a row of 8192 in documents,
+// 12 heads of 64, 90, the time of its longest document; 8 x 512 with slopes in fp32 58; 24 tokens 6.
 #include "common.h"
 #include "kernels.h"
 #include "lds_dma.h"
@@ -157,12 +165,15 @@ __device__ __forceinline__ WaveKeys wave_keys(KeyRange r, bool row) {
 // largest. The softmax does not depend on either.
 constexpr float kSlack = 8.0f, kLift = 6.0f;
 
+// Up to this cap fp16 scores may be off by 2^-22 of it: at most 2^-14, and a probability by an eighth of its
+// rounding to fp16.
+constexpr float kCoarseCap = 256.0f;
+
 // What the kernels on tiles take beside the arguments: signs and factors of the scores in log2 units.
 struct ScoreArgs {
   float q_sign;  // -1 for a negative scale, 0 for none
   float scale2;  // |scale| log2 e; with a cap the factor in front of tanh's exponent, 2 |scale| log2 e / cap
   float cap2;    // cap log2 e
-  bool coarse;   // the cap's tanh may be off by 2^-23 of the cap rather than of the score
 };
 
 // tanh of half of x ln 2, to about 4 units of 2^-24 relative: t / (t + 2) of t = 2^x - 1 = 2^n (2^f - 1) + 2^n - 1 with
@@ -186,8 +197,10 @@ __device__ __forceinline__ float tanh_of_log2(float x) {
 // What is done to the products before the softmax: nothing (they are scaled as exponents are taken), the cap
 // alone, or a cap or none and then a bias, told apart as the kernel runs. (With the cap alone told apart there
 // too, 2 x 4096 with 16 heads of 128, a cap and a window took 143 us instead of 119.)
-// fp16 takes kCapped where the tanh may be coarse.
-enum class Scores { kPlain, kCapped, kAny };
+// fp16 takes kCapped and kAny where the tanh may be coarse, else kAnyFine (within kAny it cost a third wavefront a
+// SIMD at 96 channels: 8 x 1024, 16 heads, with slopes 93 -> 102 us).
+enum class Scores { kPlain, kCapped, kAny, kAnyFine };
+constexpr bool any(Scores how) { return how == Scores::kAny || how == Scores::kAnyFine; }
 
 // Scores of one 32-key block, from products to log2 units, still to be masked: element e of lane (query, h)
 // is the key 8 (e / 4) + 4 h + e % 4 of the block. rel: the key of element 0 less the query's position.
@@ -195,7 +208,7 @@ template <bool F16, Scores HOW>
 __device__ __forceinline__ void score_block(floatx16& v, const MaskedArgs& a, const ScoreArgs& s,
                                             float slope2, float rel, const float* biases) {
   // tanh(u) = 1 - 2 / (exp(2 u) + 1): exact at both ends, off by at most 2^-23 around 0. Under fp16 probabilities
-  // (2^-11) that is nothing for the caps that coarse stands for; fp32 takes the tanh that is exact there too.
+  // (2^-11) that is nothing for caps up to kCoarseCap; fp32 takes the tanh that is exact there too.
   auto turned = [&](float x) {
     return -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * s.scale2) + 1.0f);
   };
@@ -206,7 +219,7 @@ __device__ __forceinline__ void score_block(floatx16& v, const MaskedArgs& a, co
     return;
   }
   if (a.cap > 0.0f) {
-    if (F16 && s.coarse) {
+    if constexpr (F16 && HOW == Scores::kAny) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = fmaf(2.0f * s.cap2, turned(v[e]), s.cap2);
     } else {
@@ -481,12 +494,12 @@ struct Tile {
 //   S^T: step s takes channels s and s + DP / 2, so that a lane's values of Q are neighbours.
 //   O^T: the two keys of step e are those of the lanes' element e.
 template <bool F16, int DP, int KS, Scores HOW>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Scores::kAny || DP < 128 : DP == 64) ? 3 : 2) void attn_masked_tiles(MaskedArgs a, ScoreArgs sc) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? !any(HOW) || DP < 128 : DP == 64) ? 3 : 2) void attn_masked_tiles(MaskedArgs a, ScoreArgs sc) {
   using T = Tile<F16, DP, KS>;
   using E = typename T::T;
   constexpr int KT = T::KT, QB = 128 / KS, NDT = DP / 32, NST = T::NST;
   constexpr int JOIN = (KS - 1) * (4 / KS) * Softmax<NDT>::BOX * 256;
-  constexpr int BIAS_BYTES = HOW == Scores::kAny ? 2 * T::BIASES * 4 : 0;
+  constexpr int BIAS_BYTES = any(HOW) ? 2 * T::BIASES * 4 : 0;
   constexpr int BYTES = T::RING + BIAS_BYTES > JOIN ? T::RING + BIAS_BYTES : JOIN;
   __shared__ __attribute__((aligned(1024))) char lds[BYTES];
   __shared__ int ends[4][2];
@@ -509,8 +522,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Score
   }
   // what a score is multiplied by as its exponent is taken
   const float factor = HOW == Scores::kPlain ? sc.scale2 : HOW == Scores::kCapped ? (F16 ? 2.0f : 1.0f) * sc.cap2 : 1.0f;
-  const bool tabled = HOW == Scores::kAny && a.bias_kind == kBiasTable;
-  const float slope2 = HOW == Scores::kAny && a.bias_kind == kBiasSlopes ? a.bias[w.head] * kLog2e : 0.0f;
+  const bool tabled = any(HOW) && a.bias_kind == kBiasTable;
+  const float slope2 = any(HOW) && a.bias_kind == kBiasSlopes ? a.bias[w.head] * kLog2e : 0.0f;
   const float* const table = a.bias + w.head * (2 * static_cast<size_t>(a.radius) + 1);  // if tabled
   w.look(a);
   if (lane == 0) {
@@ -630,7 +643,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : KS == 1 && (F16 ? HOW != Score
 #pragma unroll
       for (int nb = 0; nb < T::NB; ++nb) {
         auto probability = [&](int e) {
-          return __builtin_amdgcn_exp2f(HOW == Scores::kAny ? s[nb][e] - soft.base : fmaf(s[nb][e], factor, -soft.base));
+          return __builtin_amdgcn_exp2f(any(HOW) ? s[nb][e] - soft.base : fmaf(s[nb][e], factor, -soft.base));
         };
         const int kn = kb + 32 * nb;
         if constexpr (F16) {
@@ -687,7 +700,7 @@ hipError_t launch_tiles(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st)
   constexpr int QB = 128 / KS;
   const dim3 grid(static_cast<unsigned>(static_cast<uint64_t>(a.B) * a.H * ((a.S + QB - 1) / QB)));
   if constexpr (F16 || DP < 256 || KS == 1)
-    if (a.bias_kind != kBiasNone || (F16 && a.cap > 0.0f && !s.coarse)) {
+    if (a.bias_kind != kBiasNone) {
       attn_masked_tiles<F16, DP, KS, Scores::kAny><<<grid, 256, 0, st>>>(a, s);
       return hipGetLastError();
     }
@@ -714,6 +727,12 @@ hipError_t launch_tiles(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st)
 //     beyond                              fp16 26 x 402, 4 heads of 256, W 416     49.1  59.4   -
 template <bool F16, int DP>
 hipError_t launch_split(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st) {
+  if constexpr (F16)
+    if (a.cap > kCoarseCap) {
+      attn_masked_tiles<F16, DP, 1, Scores::kAnyFine>
+          <<<dim3(static_cast<unsigned>(static_cast<uint64_t>(a.B) * a.H * ((a.S + 127) / 128))), 256, 0, st>>>(a, s);
+      return hipGetLastError();
+    }
   constexpr bool FILLS = DP == 256 || (!F16 && DP >= 96);
   const int64_t w = int64_t{a.B} * a.H * ((a.S + 127) / 128);
   const int64_t reach = a.window ? std::min<int64_t>(a.S, 2 * int64_t{a.window} + 128) : a.S;
@@ -748,8 +767,6 @@ hipError_t launch_attention_masked(const MaskedArgs& a, hipStream_t st) {
   s.q_sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
   s.scale2 = a.cap > 0.0f ? 2.0f * size / a.cap : a.scale == 0.0f ? 1.0f : size;
   s.cap2 = a.cap * kLog2e;
-  // a score is then off by at most 256 x 2^-22 = 2^-14, its probability by an eighth of its rounding to fp16
-  s.coarse = a.f16 && a.cap <= 256.0f;
   return a.f16 ? launch_sized<true>(a, s, st) : launch_sized<false>(a, s, st);
 }
 

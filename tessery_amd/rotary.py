@@ -64,11 +64,16 @@ def table(runtime: HipRuntime, *, positions: int, dim: int, theta: float = 1e6,
             not np.isfinite(values).all():
         raise InferenceError()
     source = runtime.upload(values)
+    made = None
     try:
         made = runtime.buffer(positions * dim * 4)
         with runtime.command():
             runtime._rotary_table([source, made], positions=positions, rotary_dim=dim,
                                   factor=multiplier)
         return made
+    except BaseException:
+        if made is not None:
+            made.close()
+        raise
     finally:
         source.close()
