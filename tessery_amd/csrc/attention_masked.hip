@@ -13,7 +13,7 @@
 // which bound it beside them: uniform rows of 8192, 16 fp16 heads of 128, run at about 800 TFLOP/s, of 2048, 48
 // heads of 64, at 670, in fp32 32 heads of 64 at 104 (a product of 8192^3 reaches 1355 and 153). 2 x 4096 with a cap
 // and a window of 1024 takes 116 us, of which the cap's two transcendentals are about a third; a row of 8192 in documents,
-// 12 heads of 64, 90, the time of its longest document; 8 x 512 with slopes in fp32 58; 24 tokens 6.
+// 12 heads of 64, 80, two rounds of workgroups of unlike length; 8 x 512 with slopes in fp32 58; 24 tokens 6.
 #include "common.h"
 #include "kernels.h"
 #include "lds_dma.h"
@@ -104,6 +104,16 @@ __device__ __forceinline__ void masked_row(const MaskedArgs& a, int b, int i, in
     if (lane + 64 * c < a.D) out[lane + 64 * c] = static_cast<T>(acc[c] * inv);
 }
 
+// Batch rows of a few tokens: a wavefront for each token and head, instead of a tile that is mostly masked.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_masked_rows(MaskedArgs a) {
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= static_cast<uint32_t>(a.B) * a.S * a.H) return;  // wavefront-uniform
+  const uint32_t token = row / a.H;
+  masked_row<T>(a, static_cast<int>(token / a.S), static_cast<int>(token % a.S), static_cast<int>(row % a.H),
+                threadIdx.x & 63);
+}
+
 // 8 bytes of a row-major fp16 V tile a lane, transposed across each group of 16 lanes: lane r of a group
 // names row r / 4, channels 4 (r % 4) .. + 3 and receives channel r of the four rows.
 typedef __fp16 fp16x4_t __attribute__((ext_vector_type(4)));
@@ -169,6 +179,17 @@ constexpr float kSlack = 8.0f, kLift = 6.0f;
 // rounding to fp16.
 constexpr float kCoarseCap = 256.0f;
 
+// Blocks of queries of a batch row, up to which those of long documents come first. It takes about 1 us, and so is
+// left out where all workgroups run at once: 1 x 8192 in documents, 12 heads of 64 (1536 workgroups), 90 -> 78 us, fp32
+// 8 x 2002, 12 heads of 40, 462 -> 393; 4 x 246, 36 heads of 128, 64 -> 67.
+constexpr int kRanked = 256;
+
+// Rows of up to so many tokens go to attn_masked_rows, of twice as many where a tile's work is largest (256
+// channels, fp32 above 64). 512 x S, 16 heads on 8, as rows and in tiles, us: 128 fp16, S = 1 8.2 and 58.9, S = 4 29.6
+// and 59.5, S = 8 116 and 60; 256 fp32, S = 1 9.4 and 479, S = 8 179 and 484, S = 16 820 and 504; one of them: 128 fp16,
+// S = 4 8.0 and 7.9; 256 fp32, S = 8 13.7 and 18.5.
+constexpr int kFewTokens = 4;
+
 // What the kernels on tiles take beside the arguments: signs and factors of the scores in log2 units.
 struct ScoreArgs {
   float q_sign;  // -1 for a negative scale, 0 for none
@@ -178,10 +199,8 @@ struct ScoreArgs {
 
 // tanh of half of x ln 2, to about 4 units of 2^-24 relative: t / (t + 2) of t = 2^x - 1 = 2^n (2^f - 1) + 2^n - 1 with
 // n the integer next to x, where 2^f - 1 is a polynomial (minimax of the relative error on [-1/2, 1/2], 2^-25).
-// Keeps NaN.
+// NaN for NaN and infinities, whose rows are then made by masked_row.
 __device__ __forceinline__ float tanh_of_log2(float x) {
-  x = x > 64.0f ? 64.0f : x;
-  x = x < -64.0f ? -64.0f : x;
   const float n = rintf(x), f = x - n;
   float p = 0x1.39f2eap-13f;
   p = fmaf(p, f, 0x1.5e8ac4p-10f);
@@ -189,7 +208,8 @@ __device__ __forceinline__ float tanh_of_log2(float x) {
   p = fmaf(p, f, 0x1.c6b084p-5f);
   p = fmaf(p, f, 0x1.ebfbe0p-3f);
   p = fmaf(p, f, 0x1.62e430p-1f) * f;
-  const float two = __builtin_amdgcn_ldexpf(1.0f, static_cast<int>(n));
+  // from 2^64 on t / (t + 2) is 1, and -1 from 2^-64 - 1
+  const float two = __builtin_amdgcn_ldexpf(1.0f, static_cast<int>(__builtin_amdgcn_fmed3f(n, -64.0f, 64.0f)));
   const float t = fmaf(two, p, two - 1.0f);
   return t * __builtin_amdgcn_rcpf(t + 2.0f);
 }
@@ -254,6 +274,38 @@ __device__ __forceinline__ int row_of_rank(const MaskedArgs& a, int rank) {
   return __ffsll(__ballot(lane < a.B && before == rank)) - 1;
 }
 
+// The block of QB queries of batch row b that comes `place`-th by the span of keys from its first token's to its
+// last one's (powers of two from 128 keys on; equal ones from the last).
+template <int QB>
+__device__ __forceinline__ int block_by_span(const MaskedArgs& a, int b, int blocks, int place) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t* const spans = a.spans + 2 * static_cast<size_t>(b) * a.S;
+  int size[kRanked / 64];
+#pragma unroll
+  for (int m = 0; m < kRanked / 64; ++m) {
+    const int n = lane + 64 * m;
+    size[m] = -1;
+    if (n < blocks) {
+      const uint32_t lo = min(spans[2 * n * QB], static_cast<uint32_t>(a.S));
+      const uint32_t hi = min(spans[2 * min(n * QB + QB - 1, a.S - 1) + 1], static_cast<uint32_t>(a.S));
+      const uint32_t keys = hi > lo ? hi - lo : 0;
+      size[m] = keys < 128 ? 0 : min(24 - __clz(static_cast<int>(keys)) + 1, 7);
+    }
+  }
+  for (int k = 7; k >= 0; --k)
+#pragma unroll
+    for (int m = kRanked / 64 - 1; m >= 0; --m) {
+      const unsigned long long mask = __ballot(size[m] == k);
+      const int count = __popcll(mask);
+      if (place < count) {
+        const int above = count - 1 - static_cast<int>(__popcll(mask & ((1ull << lane) - 1)));
+        return __ffsll(__ballot(size[m] == k && above == place)) - 1 + 64 * m;
+      }
+      place -= count;
+    }
+  return 0;
+}
+
 // Where a workgroup of four wavefronts works: 4 / KS wavefronts of 32 queries of one head each, in KS
 // groups that share the keys out. Lane l holds query r = l % 32, as its half h = l / 32.
 template <int KS>
@@ -273,7 +325,7 @@ struct Place {
     qw = wave % QW;
     group = wave / QW;
     // Long work first: batch rows by falling length, blocks of queries from the last (under a causal mask the
-    // longest, and outermost there). Within that, key heads change fastest, so that neighbours, which start
+    // longest, and outermost there), or by the documents they meet. Within that, key heads change fastest, so that neighbours, which start
     // on different compute units, are alike, and where they are a multiple of eight the query heads of one
     // meet on one XCD.
     const int blocks = (a.S + QB - 1) / QB, share = a.H / a.KV;
@@ -290,8 +342,10 @@ struct Place {
       rank = at % a.B;
       block = at / a.B;
     }
-    const int qb = blocks - 1 - block;
     b = row_of_rank(a, rank);
+    const bool ranked = a.spans && blocks >= 16 && blocks <= kRanked && gridDim.x >= 768;
+    const int qb = ranked ? __builtin_amdgcn_readfirstlane(block_by_span<QB>(a, b, blocks, block))
+                          : blocks - 1 - block;
     i0 = qb * QB;
     i = i0 + qw * 32 + r;
     row = i < a.S;
@@ -721,7 +775,7 @@ hipError_t launch_tiles(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st)
 //                                         fp32 8 x 1589, 4 heads of 32, causal     95.8  71.3  77.8
 //     beyond                              fp16 5 x 1971, 8 heads of 64, W 640      64.1  76.0  94.2
 //   twice that with spans, up to 64 channels or from 96 in fp32 (a block's documents may lie far apart)
-//                                         fp16 1 x 8192, 12 heads of 64           103    89     -
+//                                         fp16 1 x 8192, 12 heads of 64           103    80     -
 //   W <= 256 where one workgroup's tiles fill a compute unit (fp32 from 96 channels, 256 channels)
 //                                         fp32 10 x 1518, 4 heads of 128          208   120     -
 //     beyond                              fp16 26 x 402, 4 heads of 256, W 416     49.1  59.4   -
@@ -757,11 +811,19 @@ hipError_t launch_sized(const MaskedArgs& a, const ScoreArgs& s, hipStream_t st)
 }  // namespace
 
 bool attention_masked_fits(uint64_t B, uint64_t S, uint64_t H, uint64_t D) {
-  // a launch's work items stay below 2^32
+  // a launch's work items stay below 2^32: attn_masked_rows has 64 for a row; with more tokens than it takes, a
+  // block of queries has 256
+  static_assert(kFewTokens >= 4, "2^26 / 5 blocks of 256 work items");
   return D % 8 == 0 && D <= 256 && B * S * H < (1ull << 26);
 }
 
 hipError_t launch_attention_masked(const MaskedArgs& a, hipStream_t st) {
+  if (a.S <= (a.D > 128 || (!a.f16 && a.D > 64) ? 2 * kFewTokens : kFewTokens)) {
+    const dim3 grid(static_cast<unsigned>((static_cast<uint64_t>(a.B) * a.S * a.H + 3) / 4));
+    if (a.f16) attn_masked_rows<_Float16><<<grid, 256, 0, st>>>(a);
+    else attn_masked_rows<float><<<grid, 256, 0, st>>>(a);
+    return hipGetLastError();
+  }
   const float size = fabsf(a.scale) * kLog2e;
   ScoreArgs s{};
   s.q_sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;

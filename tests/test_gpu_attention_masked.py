@@ -274,12 +274,51 @@ def test_many_and_few_workgroups(runtime, precision, b, s, h, kv, d):
 
 
 @pytest.mark.parametrize("precision", ["f16", "f32"])
+@pytest.mark.parametrize("d", [8, 64, 72, 128, 136, 256])
+@pytest.mark.parametrize("s", [1, 2, 4, 5, 8, 9])
+def test_a_few_tokens(runtime, precision, d, s):
+    """Batch rows on either side of the lengths that go without tiles."""
+    q, k, v = operands(31, 7, s, 6, 2, d, precision)
+    lengths = np.random.default_rng(31).integers(0, s + 1, size=7)
+    check(runtime, q, k, v, lengths, mask="causal")
+    check(runtime, q, k, v, lengths, mask="prefix", prefix=lengths[::-1].copy(), cap=5.0, packed=True)
+    check(runtime, q, k, v, lengths, mask="bidirectional", window=2,
+          slopes=np.array([0.1, 0.02, 0.3, 0.0, 1.0, 0.5], np.float32))
+    table = np.random.default_rng(32).standard_normal((6, 7)).astype(np.float32)
+    check(runtime, q, k, v, lengths, mask="causal", table=table,
+          spans=batching.document_spans([[s // 2, s - s // 2] if s > 1 else [1]] * 7, s))
+
+
+def test_very_many_single_tokens(runtime):
+    """The weight of a lone key is one: a row is its value, to the last of 2^24."""
+    many, v = 2**19, np.random.default_rng(33).standard_normal((2**19, 1, 1, 8)).astype(np.float16)
+    q = np.ones((many, 1, 32, 8), np.float16)
+    got = run(runtime, q, v, v, np.ones(many, np.uint32), mask="causal")
+    np.testing.assert_array_equal(got, np.broadcast_to(v, got.shape))
+
+
+@pytest.mark.parametrize("precision", ["f16", "f32"])
 def test_all_at_once(runtime, precision):
     q, k, v = operands(19, 2, 260, 8, 4, 128, precision)
     table = np.random.default_rng(19).standard_normal((8, 65)).astype(np.float32)
     check(runtime, q, k, v, [260, 131], mask="prefix", prefix=np.array([30, 200]), window=90,
           cap=25.0, table=table, packed=True,
           spans=batching.document_spans([[100, 160], [131]], 260))
+
+
+@pytest.mark.parametrize("precision", ["f16", "f32"])
+@pytest.mark.parametrize("mask", ["causal", "bidirectional"])
+@pytest.mark.parametrize("spans", ["documents", "anything"])
+def test_many_blocks_of_documents(runtime, precision, mask, spans):
+    """So many workgroups that blocks of long documents come first: each block is one's, whatever the
+    spans hold."""
+    q, k, v = operands(34, 2, 1090, 48, 24, 8, precision)
+    if spans == "documents":
+        at = batching.document_spans([[7, 500, 64, 1, 128, 300, 90], [1, 1, 700, 20]], 1090)
+    else:
+        at = np.random.default_rng(35).integers(0, 1300, size=(2, 1090, 2)).astype(np.uint32)
+        at[0, ::64], at[1, 63::64] = (0, 2**32 - 1), (2**32 - 1, 0)
+    check(runtime, q, k, v, [1090, 722], mask=mask, spans=at)
 
 
 def test_a_long_row_of_documents(runtime):
